@@ -1,0 +1,416 @@
+// The weight that every cached token collects from a prompt's tokens, on tcgen05:
+//     mass[row, kvh, j] += sum over the tokens i and the query heads of the group of exp(x_ij - lse_i)
+// with the scores of shaped.cuh and the log-sum-exp that the attention pass left.
+//
+// A CTA takes NT tiles of 128 keys of one KV head as the left operand, so that a key is a lane of the tensor memory and a thread adds up its
+// own key's weight: no reduction across threads, no atomics, one order of the sum.  The query rows that may see the keys stream
+// through a ring in steps of 128 (tokens x heads of the group), with their log-sum-exp, positions, bounds and slopes as columns in shared memory:
+//     S_t = K_t Q^T      UMMA 128 x 128 x D, two buffers per key tile in tensor memory
+//     sum                four warps per key tile: exp2(x - lse) of 128 columns, masked by the key's position where a column does not see all keys
+// What bounds it is the exponential, one per (token, head, key) pair; the product is half of the attention's.
+// The grid is persistent: key tiles of all sequences, those with most tokens behind them first.
+#include "shaped.cuh"
+
+namespace smc {
+
+constexpr int MS_LOADERS = 4, MS_Q = 128;
+
+template <int D> struct MsCfg;                        // key tiles of a CTA, slots of the ring of query steps, of them in flight
+template <> struct MsCfg<64> { static constexpr int NT = 2, QU = 6, LAG = 3; };
+template <> struct MsCfg<128> { static constexpr int NT = 2, QU = 4, LAG = 2; };
+template <> struct MsCfg<256> { static constexpr int NT = 1, QU = 2, LAG = 1; };
+
+struct ShapedMassParams {
+  ShapedCache c;
+  const __nv_bfloat16* q;
+  const __nv_bfloat16* k_pool;
+  const int4* runs;
+  const float* lse;              // [T, Hq]
+  float* mass;                   // [bt_rows, Hkv, mass_stride]
+  long long ld_q, mass_stride;
+  int n_runs, T, Hq, Hkv, pdl;
+  int* status;
+};
+
+// What a step's query rows bring along, by column
+struct alignas(16) MsColumns {
+  float neg_lse[MS_Q], pos[MS_Q], first[MS_Q], last[MS_Q], slope[MS_Q];
+  float max_first[4], min_last[4];                    // over 32 columns each: a key between all of them is seen by every column
+};
+
+template <int D> struct MsShared {
+  static constexpr int SLOTS = MsCfg<D>::QU + 2;      // a step's columns are read until its sums are done, two products behind the ring
+  MsColumns col[SLOTS];
+  uint64_t q_full[MsCfg<D>::QU], q_empty[MsCfg<D>::QU], col_full[SLOTS], k_full, s_full[2][2], s_empty[2][2];
+  uint32_t tmem_slot;
+  int lo[16], hi[16];
+  volatile int abort;
+};
+
+template <typename Shared>
+__device__ __forceinline__ bool ms_wait(Shared& S, int* status, uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (S.abort) return false;
+    if (clock64() - t0 > SMC_SPIN_CYCLES) {
+      atomicOr(status, SMC_ERR_BARRIER_TIMEOUT);
+      S.abort = 1;
+      return false;
+    }
+  }
+}
+
+// All tiles of `kt` keys of all sequences, those with most tokens behind their first key in front; used by whole warps.
+struct MsTiles {
+  const ShapedMassParams& p;
+  int kt;
+  ShapedRun mine;
+  __device__ MsTiles(const ShapedMassParams& params, int keys) : p(params), kt(keys) { mine = run_of((int)threadIdx.x & 31); }
+  __device__ ShapedRun run_of(int s) const { return s < p.n_runs ? shaped_run(p.c, p.runs, s, p.T, p.status) : ShapedRun{0, 0, 0, 0}; }
+  // tiles of run r with at least `tokens` of its new tokens at or behind their first key: the first ones of the row
+  __device__ int of_run(const ShapedRun& r, int tokens) const { return tokens > r.n ? 0 : (r.held + r.n - tokens) / kt + 1; }
+  __device__ long long count(int tokens) const {
+    int n = of_run(mine, tokens);
+    for (int s = (threadIdx.x & 31) + 32; s < p.n_runs; s += 32) n += of_run(run_of(s), tokens);
+    return (long long)__reduce_add_sync(0xffffffffu, (unsigned)n);
+  }
+  // tile number `want`: its run, the run's number and the tile inside it
+  __device__ bool find(long long want, ShapedRun& run, int& number, int& tile) const {
+    const int lane = threadIdx.x & 31;
+    int lo = 1, hi = p.T + 1;                         // count(lo) > want >= count(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (count(mid) > want) lo = mid; else hi = mid;
+    }
+    int left = (int)(want - count(lo + 1));
+    for (int s0 = 0; s0 < p.n_runs; s0 += 32) {
+      const ShapedRun r = s0 == 0 ? mine : run_of(s0 + lane);
+      const int more = of_run(r, lo + 1), n = of_run(r, lo) - more;
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += up;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, left >= sum - n && left < sum);
+      if (hit) {
+        const int src = __ffs(hit) - 1;
+        run.row = __shfl_sync(0xffffffffu, r.row, src);
+        run.held = __shfl_sync(0xffffffffu, r.held, src);
+        run.at = __shfl_sync(0xffffffffu, r.at, src);
+        run.n = __shfl_sync(0xffffffffu, r.n, src);
+        tile = __shfl_sync(0xffffffffu, more + left - (sum - n), src);
+        number = s0 + src;
+        return true;
+      }
+      left -= __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return false;
+  }
+};
+
+template <int D, bool CAP, bool BIAS>
+__global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shaped_mass_kernel(const ShapedMassParams p) {
+  constexpr int NT = MsCfg<D>::NT, QU = MsCfg<D>::QU, LAG = MsCfg<D>::LAG;
+  constexpr int NPAN = D / 64, PANEL = 128 * 128, TILE = NPAN * PANEL, CPR = D / 8;
+  using Shared = MsShared<D>;
+  constexpr int SLOTS = Shared::SLOTS;
+  extern __shared__ uint8_t ms_smem_raw[];
+  __shared__ Shared S;
+  const uint32_t raw = smem_u32(ms_smem_raw);
+  uint8_t* smem = ms_smem_raw + (((raw + 1023u) & ~1023u) - raw);
+  uint8_t* k_s = smem;                                // [NT] keys
+  uint8_t* q_s = smem + NT * TILE;                    // [QU] query steps
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr int LOAD_WARP = 4 * NT, MMA_WARP = LOAD_WARP + MS_LOADERS;
+  const int G = p.Hq / p.Hkv, TT = 128 / G;           // tokens of a step
+  if (warp == MMA_WARP) {
+    tmem_alloc(&S.tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < QU; ++i) {
+      mbar_init(&S.q_full[i], MS_LOADERS);
+      mbar_init(&S.q_empty[i], NT);
+    }
+    for (int i = 0; i < SLOTS; ++i) mbar_init(&S.col_full[i], MS_LOADERS);
+    mbar_init(&S.k_full, MS_LOADERS);
+    for (int t = 0; t < NT; ++t)
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&S.s_full[t][i], 1);
+        mbar_init(&S.s_empty[t][i], 4);
+      }
+    S.abort = 0;
+    fence_barrier_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = S.tmem_slot;
+  if (p.pdl) { pdl_launch_dependents(); pdl_wait_prior_grid(); }
+
+  const MsTiles all(p, NT * 128);
+  const long long items = all.count(1) * p.Hkv;
+  bool dead = false;                                  // a wait of this warp ran out: it goes on to the end without work
+  uint32_t u0 = 0, k_use = 0;                         // steps and key tiles so far: barriers run on from item to item
+  for (long long base = 0, round = 0; base < items; base += gridDim.x, ++round) {
+    // every second round runs backwards, so that who had a long tile gets a short one
+    const long long item = base + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    ShapedRun run{0, 0, 0, 0};
+    int number = 0, tile = 0;
+    bool have = item < items && all.find(item / p.Hkv, run, number, tile);
+    if (have) {
+      bool twice = false;                             // a row listed twice would be added to by two blocks at once
+      for (int o = lane; o < number; o += 32) twice |= p.runs[o].x == run.row && p.runs[o].w > 0;
+      if (__any_sync(0xffffffffu, twice)) {
+        if (threadIdx.x == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
+        have = false;
+      }
+    }
+    const int kvh = (int)(item % p.Hkv), hbase = kvh * G, keys = run.held + run.n, k0 = tile * NT * 128;
+    const int* kp = p.c.key_pos != nullptr ? p.c.key_pos + (size_t)run.row * p.c.kp_stride : nullptr;
+    auto pos_of = [&](int idx) { return kp != nullptr ? kp[idx] : idx; };
+    // new tokens [ta, tb) of the run that may see one of the keys
+    int ta = max(0, k0 - run.held), tb = have ? run.n : 0;
+    if (p.c.bounds != nullptr) {
+      int lo = run.n, hi = 0;
+      if (have) {
+        const int near = pos_of(k0), far = pos_of(min(k0 + NT * 128, keys) - 1);
+        for (int i = threadIdx.x; i < run.n; i += blockDim.x) {
+          const int2 b = shaped_bounds(p.c, run.at + i, 0);
+          if (b.x <= far && b.y >= near && b.x <= b.y) { lo = min(lo, i); hi = max(hi, i + 1); }
+        }
+      }
+      lo = __reduce_min_sync(0xffffffffu, lo);
+      hi = __reduce_max_sync(0xffffffffu, hi);
+      __syncthreads();                                // the item before has read its range
+      if (lane == 0) { S.lo[warp] = lo; S.hi[warp] = hi; }
+      __syncthreads();
+      ta = run.n;
+      tb = 0;
+      for (int w = 0; w < (int)(blockDim.x >> 5); ++w) { ta = min(ta, S.lo[w]); tb = max(tb, S.hi[w]); }
+    }
+    const int n_steps = tb > ta ? (tb - ta + TT - 1) / TT : 0;
+    if (n_steps == 0 || dead) continue;
+
+    if (warp >= LOAD_WARP && warp < MMA_WARP) {
+      // ================================================================= loaders
+      const int lw = warp - LOAD_WARP;
+      bool go = u0 == 0 || ms_wait(S, p.status, &S.q_empty[(u0 - 1) % QU], ((u0 - 1) / QU) & 1u);      // products with the keys before are done
+      go = __all_sync(0xffffffffu, go);
+      if (!go) { dead = true; continue; }
+      {                                               // keys: this warp's 32 of each tile
+        const int* bt = p.c.block_table + (size_t)run.row * p.c.bt_stride;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const int mine = k0 + t * 128 + lw * 32 + lane;
+          int page = mine < keys ? bt[mine] : -1;
+          if (page > p.c.n_pages || (page < 0 && mine < keys)) { atomicOr(p.status, SMC_ERR_BOUNDS); page = 0; }
+          const uint32_t dst0 = smem_u32(k_s + t * TILE);
+#pragma unroll 4
+          for (int idx = lane; idx < 32 * CPR; idx += 32) {
+            const int kl = idx / CPR, c = idx % CPR, r = lw * 32 + kl;
+            const int pg = __shfl_sync(0xffffffffu, page, kl);
+            const uint32_t dst = dst0 + (uint32_t)((c >> 3) * PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p.k_pool + (size_t)max(pg, 0) * p.Hkv * D + (size_t)kvh * D + c * 8), "r"(pg >= 0 ? 16 : 0) : "memory");
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      }
+      for (int j = 0; j < n_steps; ++j) {
+        const uint32_t u = u0 + j, st = u % QU;
+        // this lane's column
+        const int cl = lw * 32 + lane, tok = ta + j * TT + cl / G, h = hbase + cl % G;
+        const bool live = cl < TT * G && tok < tb;
+        float nl = -INFINITY, posf = 0.f, first = 0.f, last = (float)SH_POS_END, slope = 0.f;
+        if (live) {
+          const float lse = p.lse[(size_t)(run.at + tok) * p.Hq + h];
+          const int pos = pos_of(run.held + tok);
+          int2 b = shaped_bounds(p.c, run.at + tok, pos);
+          if (lse == -INFINITY) b = make_int2(SH_POS_END, -1);        // it has seen nothing
+          else nl = -lse * SH_LOG2E;
+          posf = (float)pos;
+          first = (float)b.x;
+          last = (float)b.y;
+          if (BIAS) slope = -p.c.slopes[h] * SH_LOG2E;
+        }
+        const bool ok = u < QU || ms_wait(S, p.status, &S.q_empty[st], (u / QU - 1) & 1u);
+        if (!__all_sync(0xffffffffu, ok)) { go = false; break; }
+        MsColumns& col = S.col[u % SLOTS];
+        col.neg_lse[cl] = nl;
+        col.pos[cl] = posf;
+        col.first[cl] = first;
+        col.last[cl] = last;
+        if (BIAS) col.slope[cl] = slope;
+        const float mf = warp_max(first), ml = -warp_max(-last);
+        if (lane == 0) { col.max_first[lw] = mf; col.min_last[lw] = ml; }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.col_full[u % SLOTS]);
+        const uint32_t dst0 = smem_u32(q_s + (size_t)st * TILE);
+#pragma unroll 4
+        for (int idx = lane; idx < 32 * CPR; idx += 32) {
+          const int rl = idx / CPR, c = idx % CPR, r = lw * 32 + rl, tk = ta + j * TT + r / G;
+          const bool real = r < TT * G && tk < tb;
+          const __nv_bfloat16* src = p.q + (size_t)(run.at + (real ? tk : ta)) * p.ld_q + (size_t)(hbase + r % G) * D + c * 8;
+          const uint32_t dst = dst0 + (uint32_t)((c >> 3) * PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (j >= LAG - 1) {                           // the keys, then step j - LAG, have landed: hand them over
+          asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(j == LAG - 1 ? &S.k_full : &S.q_full[(u - LAG) % QU]);
+        }
+      }
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      fence_proxy_async();
+      __syncwarp();
+      if (!go) { dead = true; continue; }
+      if (lane == 0) {
+        if (n_steps < LAG) mbar_arrive(&S.k_full);
+        for (int j = max(0, n_steps - LAG); j < n_steps; ++j) mbar_arrive(&S.q_full[(u0 + j) % QU]);
+      }
+    } else if (warp >= MMA_WARP) {
+      // ================================================================= MMA issuers (one thread per key tile)
+      const int t = warp - MMA_WARP;
+      bool ok = true;
+      if (elect_one()) {
+        constexpr uint32_t idesc = umma_idesc_bf16(128, MS_Q);
+        const uint32_t k_addr = smem_u32(k_s) + t * TILE;
+        ok = ms_wait(S, p.status, &S.k_full, k_use & 1u);
+        for (int j = 0; ok && j < n_steps; ++j) {
+          const uint32_t u = u0 + j, st = u % QU, buf = u & 1u;
+          ok = ms_wait(S, p.status, &S.q_full[st], (u / QU) & 1u) && (u < 2 || ms_wait(S, p.status, &S.s_empty[t][buf], (u / 2 - 1) & 1u));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t q_addr = smem_u32(q_s + (size_t)st * TILE);
+#pragma unroll
+          for (int pan = 0; pan < NPAN; ++pan)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16_ss(tmem_base + (uint32_t)(t * 2 + buf) * 128u, umma_desc_k_sw128(k_addr + pan * PANEL) + 2 * k,
+                           umma_desc_k_sw128(q_addr + pan * PANEL) + 2 * k, idesc, (pan | k) ? 1u : 0u);
+          umma_commit(&S.s_full[t][buf]);
+          umma_commit(&S.q_empty[st]);
+        }
+      }
+      if (!__all_sync(0xffffffffu, ok)) { dead = true; continue; }
+    } else {
+      // ================================================================= sums (one key per thread)
+      const int t = warp >> 2, r = (warp & 3) * 32 + lane, k = k0 + t * 128 + r;
+      const uint32_t ts = tmem_base + (uint32_t)t * 256u + (((uint32_t)((warp & 3) * 32)) << 16);
+      const float kpos = k < keys ? (float)pos_of(k) : -1.f;
+      const float mul = p.c.scale * SH_LOG2E, cap_in = CAP ? p.c.scale / p.c.cap : 0.f, cap_out = CAP ? p.c.cap * SH_LOG2E : 0.f;
+      const uint64_t mul2 = f2_pair(mul, mul), kpos2 = f2_pair(kpos, kpos);
+      float total = 0.f;
+      bool alive = true;
+      for (int j = 0; j < n_steps; ++j) {
+        const uint32_t u = u0 + j, buf = u & 1u;
+        const MsColumns& col = S.col[u % SLOTS];
+        if (!__all_sync(0xffffffffu, ms_wait(S, p.status, &S.s_full[t][buf], (u / 2) & 1u) &&
+                                         ms_wait(S, p.status, &S.col_full[u % SLOTS], (u / SLOTS) & 1u))) { alive = false; break; }
+        tc_fence_after();
+        const float4 mf = *reinterpret_cast<const float4*>(col.max_first), ml = *reinterpret_cast<const float4*>(col.min_last);
+        const bool full = __all_sync(0xffffffffu, kpos >= fmaxf(fmaxf(mf.x, mf.y), fmaxf(mf.z, mf.w)) && kpos <= fminf(fminf(ml.x, ml.y), fminf(ml.z, ml.w)));
+        uint64_t part[2] = {0ull, 0ull};              // a step's sum in four parts ahead of the running one: short chains of additions
+#pragma unroll
+        for (int c0 = 0; c0 < MS_Q; c0 += 32) {
+          uint32_t w[32];
+          tmem_ld_32x32b_x16(ts + buf * 128u + c0, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
+          tmem_ld_32x32b_x16(ts + buf * 128u + c0 + 16, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
+          tmem_ld_wait();
+          uint64_t x[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) x[i] = f2_pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+          if (CAP) {
+            shaped_cap_pairs<6, 8>(*reinterpret_cast<uint64_t(*)[8]>(&x[0]), cap_in, cap_out);
+            shaped_cap_pairs<6, 8>(*reinterpret_cast<uint64_t(*)[8]>(&x[8]), cap_in, cap_out);
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const uint64_t nl = *reinterpret_cast<const uint64_t*>(&col.neg_lse[c0 + 2 * i]);
+            x[i] = CAP ? f2_add(x[i], nl) : f2_fma(x[i], mul2, nl);
+            if (BIAS) {
+              const float2 d = f2_unpair(f2_fma(*reinterpret_cast<const uint64_t*>(&col.pos[c0 + 2 * i]), f2_pair(-1.f, -1.f), kpos2));
+              x[i] = f2_fma(f2_pair(fabsf(d.x), fabsf(d.y)), *reinterpret_cast<const uint64_t*>(&col.slope[c0 + 2 * i]), x[i]);
+            }
+            const float2 v = f2_unpair(x[i]);
+            float e0 = shaped_ex2(v.x), e1 = shaped_ex2(v.y);
+            if (!full) {
+              const int c = c0 + 2 * i;
+              e0 = kpos >= col.first[c] && kpos <= col.last[c] ? e0 : 0.f;
+              e1 = kpos >= col.first[c + 1] && kpos <= col.last[c + 1] ? e1 : 0.f;
+            }
+            part[i & 1] = f2_add(part[i & 1], f2_pair(e0, e1));
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S.s_empty[t][buf]);
+        const float2 a = f2_unpair(part[0]), b = f2_unpair(part[1]);
+        total += (a.x + a.y) + (b.x + b.y);
+      }
+      if (!alive) { dead = true; continue; }
+      if (k < keys) p.mass[((size_t)run.row * p.Hkv + kvh) * p.mass_stride + k] += total;
+    }
+    u0 += n_steps;
+    ++k_use;
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem_base, 512);
+}
+
+template <int D, bool CAP, bool BIAS>
+static int launch_shaped_mass(const ShapedMassParams& p, cudaStream_t st) {
+  constexpr size_t smem = (size_t)(MsCfg<D>::NT + MsCfg<D>::QU) * D * 256 + 1024;
+  static_assert(smem + sizeof(MsShared<D>) <= 232448, "shared memory");
+  CUDA_CHECK_RET(cudaFuncSetAttribute(shaped_mass_kernel<D, CAP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(148);
+  cfg.blockDim = dim3((5 * MsCfg<D>::NT + MS_LOADERS) * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.pdl ? 1 : 0;
+  CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, shaped_mass_kernel<D, CAP, BIAS>, p));
+  return 0;
+}
+
+}  // namespace smc
+
+// q [T] rows of Hq * D bf16 values with their lse [T, Hq]; runs as in smc_shaped_prompt, every row once; mass [bt_rows, Hkv, mass_stride] fp32.
+SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, int n_pages, const int* block_table, int bt_stride, int bt_rows,
+                            const int* key_pos, int kp_stride, const int* runs, int n_runs, const float* lse, float* mass, long long mass_stride,
+                            int T, int Hq, int Hkv, int D, float scale, float cap, const float* slopes, const int* bounds, int* status, int pdl,
+                            cudaStream_t st) {
+  using namespace smc;
+  if (n_runs <= 0 || T <= 0) return 0;
+  if (Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq / Hkv > 128 || (D != 64 && D != 128 && D != 256)) return -160;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(runs)) & 15 || (ld_q & 7) ||
+      (reinterpret_cast<uintptr_t>(bounds) & 7))
+    return -161;
+  if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -162;
+  if (mass_stride < bt_stride) return -163;
+  ShapedMassParams p;
+  p.c = ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, scale, cap};
+  p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.runs = (const int4*)runs; p.lse = lse; p.mass = mass;
+  p.ld_q = ld_q; p.mass_stride = mass_stride; p.n_runs = n_runs; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.pdl = pdl; p.status = status;
+#define SMC_SHAPED_MASS(DD)                                                                                            \
+  if (D == DD) {                                                                                                       \
+    if (cap > 0.f) return slopes ? launch_shaped_mass<DD, true, true>(p, st) : launch_shaped_mass<DD, true, false>(p, st); \
+    return slopes ? launch_shaped_mass<DD, false, true>(p, st) : launch_shaped_mass<DD, false, false>(p, st);          \
+  }
+  SMC_SHAPED_MASS(64)
+  SMC_SHAPED_MASS(128)
+  SMC_SHAPED_MASS(256)
+#undef SMC_SHAPED_MASS
+  return -160;
+}
