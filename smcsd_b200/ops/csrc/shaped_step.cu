@@ -14,7 +14,10 @@
 
 namespace smc {
 
-constexpr int ST_K = 64, ST_MAX_BS = 1024, ST_PAGES = 8;
+// Registers of 384 threads, 168 each at the start: the loaders leave theirs to the warps that hold outputs.
+constexpr int ST_FEW = 40, ST_MANY = 232;
+static_assert(128 * ST_FEW + 256 * ST_MANY <= 384 * 168, "the registers of the launch");
+constexpr int ST_K = 64, ST_MAX_BS = 1024, ST_LOADERS = 4;
 constexpr int ST_COUNTERS = 32768;                     // at the front of every workspace, whatever batch it serves next
 
 struct ShapedStepParams {
@@ -135,38 +138,79 @@ __device__ __forceinline__ int step_sequence(const int* tiles, int bs, int x) {
 
 template <int D, int MT>
 struct StCfg {
-  static constexpr int WARPS = 4 * MT, LD = D + 8;                   // four groups of 16 keys x MT tiles of 16 rows
-  static constexpr int STAGES = D == 256 ? (MT == 1 ? 3 : 2) : 4;
+  // consumers: row tiles of 16 x four groups of 16 keys, twice (tiles in turn) where that makes eight warps
+  static constexpr int TURNS = MT == 1 ? 2 : 1, GROUPS = 4 * TURNS, WARPS = GROUPS * MT, THREADS = (WARPS + ST_LOADERS) * 32;
+  static constexpr int LD = D + 8;
+  static constexpr int STAGES = D == 64 ? 8 : D == 128 ? 5 : MT == 1 ? 3 : 2;
   static constexpr size_t KV = (size_t)ST_K * LD * 2;                // one of K, V
-  // stages, a state of [16 MT][D + 4] for the join, positions and pages of the tiles in flight, prefix sums
-  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)16 * MT * (D + 4) * 4 + (size_t)2 * ST_PAGES * ST_K * 4 + (ST_MAX_BS + 1 + 64) * 4;
+  // stages, a state of [16 MT][D + 4] for the join, positions of the tiles in flight, prefix sums
+  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)16 * MT * (D + 4) * 4 + (size_t)STAGES * ST_K * 4 + (ST_MAX_BS + 1 + 64) * 4;
 };
 
+// A place in the line of tiles: the sequence that tile x belongs to.
+struct StepCursor {
+  int s, seq0, seq1;
+  StepKeys key;
+  __device__ __forceinline__ void seek(const ShapedStepParams& p, const int* tiles, int x) {
+    s = step_sequence(tiles, p.bs, x);
+    seq0 = tiles[s];
+    seq1 = tiles[s + 1];
+    key = step_keys(p, s);
+  }
+};
+
+struct StShared {
+  uint64_t full[8], empty[8];
+  int last;
+  volatile int abort;
+};
+
+__device__ __forceinline__ bool st_wait(StShared& S, int* status, uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long t0 = clock64();
+  for (;;) {
+    for (int i = 0; i < 64; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (S.abort) return false;
+    if (clock64() - t0 > SMC_SPIN_CYCLES) {
+      atomicOr(status, SMC_ERR_BARRIER_TIMEOUT);
+      S.abort = 1;
+      return false;
+    }
+  }
+}
+
 template <int D, int MT>
-__global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 ? 2 : 1) shaped_step_kernel(const ShapedStepParams p) {
+__global__ void __launch_bounds__(StCfg<D, MT>::THREADS, 1) shaped_step_kernel(const ShapedStepParams p) {
   using Cfg = StCfg<D, MT>;
   constexpr int LD = Cfg::LD, STAGES = Cfg::STAGES, THREADS = Cfg::WARPS * 32, CPR = D / 8;
   extern __shared__ __align__(128) uint8_t st_smem[];
   __nv_bfloat16* kv_s = reinterpret_cast<__nv_bfloat16*>(st_smem);   // [stage][K, V][64][LD]
   float* join = reinterpret_cast<float*>(st_smem + STAGES * 2 * Cfg::KV);            // [16 MT][D + 4]
-  int* page_s = reinterpret_cast<int*>(join + 16 * MT * (D + 4));    // [ST_PAGES][64]
-  int* pos_s = page_s + ST_PAGES * ST_K;                             // [ST_PAGES][64]
-  int* tiles = pos_s + ST_PAGES * ST_K;                              // [bs + 1]
+  int* pos_s = reinterpret_cast<int*>(join + 16 * MT * (D + 4));     // [stage][64]
+  int* tiles = pos_s + STAGES * ST_K;                                // [bs + 1]
   int* misc = tiles + ST_MAX_BS + 1;                                 // [64]
-  __shared__ float ml_s[4][16 * MT][2];
-  __shared__ int last_s;
+  __shared__ float ml_s[Cfg::GROUPS][16 * MT][2];
+  __shared__ StShared S;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
-  const int mt = warp % MT, kg = warp / MT;                          // row tile, group of keys
   // rows r = token * G + head of this CTA: [m0, M)
   const int G = p.Hq / p.Hkv, m0 = blockIdx.z * 16 * MT, rows_all = p.E * G, M = min(rows_all, m0 + 16 * MT), kvh = blockIdx.y, w = blockIdx.x;
   int* counter = p.counters + ((size_t)blockIdx.z * p.bs) * p.Hkv + kvh;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&S.full[i], ST_LOADERS * 32);
+      mbar_init(&S.empty[i], 4 * MT);
+    }
+    S.abort = 0;
+    fence_barrier_init();
+  }
   if (p.pdl) { pdl_launch_dependents(); pdl_wait_prior_grid(); }
   step_schedule(p, tiles, misc);
   const int total = tiles[p.bs];
   // sequences without a tile have nobody else to write their rows
   if (w == 0) {
-    for (int s = warp; s < p.bs; s += Cfg::WARPS) {
+    for (int s = warp; s < p.bs; s += Cfg::THREADS / 32) {
       if (tiles[s + 1] > tiles[s]) continue;
       for (int x = m0 * D + lane; x < M * D; x += 32) {
         const int e = x / (G * D), hd = x - e * G * D;
@@ -183,47 +227,56 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
   if (w >= W) return;
   const int t_begin = step_first(w, W, total), t_end = step_first(w + 1, W, total);
 
-  const size_t kv_row = (size_t)p.Hkv * D;
-  const float mul = p.c.scale * SH_LOG2E, cap_in = p.c.cap > 0.f ? p.c.scale / p.c.cap : 0.f, cap_out = p.c.cap * SH_LOG2E;
-
-  // pages and positions of tile x into slot x % ST_PAGES; keys behind the last repeat it and have position -1
-  auto fetch_ids = [&](int x) {
-    if (x < t_end && threadIdx.x < ST_K) {
-      const int s = step_sequence(tiles, p.bs, x);
-      const StepKeys k = step_keys(p, s);
-      const int i = (x - tiles[s]) * ST_K + threadIdx.x, idx = k.begin + min(i, k.n - 1), slot = (x % ST_PAGES) * ST_K + threadIdx.x;
-      st_cp4(smem_u32(page_s + slot), p.c.block_table + (size_t)k.row * p.c.bt_stride + idx);
-      if (i >= k.n) pos_s[slot] = -1;
-      else if (p.c.key_pos != nullptr) st_cp4(smem_u32(pos_s + slot), p.c.key_pos + (size_t)k.row * p.c.kp_stride + idx);
-      else pos_s[slot] = idx;
+  if (warp >= Cfg::WARPS) {
+    if constexpr (D == 256) regs_fewer<ST_FEW>();
+    // ================================================================= loaders: 16 keys of each tile a warp
+    const int lw = warp - Cfg::WARPS, kl0 = lw * 16 + (lane & 15);
+    const size_t kv_row = (size_t)p.Hkv * D;
+    constexpr int AHEAD = 3;                                         // tiles that page ids are read ahead
+    StepCursor cur;
+    cur.seq1 = t_begin;
+    int page[AHEAD], from[AHEAD];                                    // of this lane's key: page, index of its position or -1
+    auto ids = [&](int x, int& pg, int& at) {
+      if (x >= t_end) return;
+      if (x >= cur.seq1) cur.seek(p, tiles, x);
+      const int i = (x - cur.seq0) * ST_K + kl0, idx = cur.key.begin + min(i, cur.key.n - 1);       // keys behind the last repeat it
+      pg = p.c.block_table[(size_t)cur.key.row * p.c.bt_stride + idx];
+      at = cur.key.row * p.c.kp_stride + idx;
+    };
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) ids(t_begin + d, page[d], from[d]);
+    for (int x0 = t_begin; x0 < t_end; x0 += AHEAD) {
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        const int x = x0 + d, n = x - t_begin, st = n % STAGES;
+        if (x >= t_end) break;
+        int pg = page[d];
+        const int at = from[d];
+        if (pg < 0 || pg > p.c.n_pages) { atomicOr(p.status, SMC_ERR_BOUNDS); pg = 0; }
+        ids(x + AHEAD, page[d], from[d]);
+        const bool ok = n < STAGES || st_wait(S, p.status, &S.empty[st], (uint32_t)(n / STAGES - 1) & 1u);
+        if (!__all_sync(0xffffffffu, ok)) { x0 = t_end; break; }
+        const uint32_t k0 = smem_u32(kv_s + (size_t)st * 2 * ST_K * LD);
+#pragma unroll 8
+        for (int i = lane; i < 16 * CPR; i += 32) {
+          const int kl = i / CPR, c = i - kl * CPR;
+          const size_t src = (size_t)__shfl_sync(0xffffffffu, pg, kl) * kv_row + (size_t)kvh * D + c * 8;
+          const uint32_t dst = k0 + (uint32_t)((lw * 16 + kl) * LD + c * 8) * 2;
+          st_cp16(dst, p.k_pool + src);
+          st_cp16(dst + (uint32_t)Cfg::KV, p.v_pool + src);
+        }
+        if (p.c.key_pos != nullptr && lane < 16) st_cp4(smem_u32(pos_s + st * ST_K + kl0), p.c.key_pos + at);
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&S.full[st])) : "memory");       // when all of them have landed
+      }
     }
-  };
-  auto fetch = [&](int x) {
-    if (x >= t_end) return;
-    const uint32_t k0 = smem_u32(kv_s + (size_t)((x - t_begin) % STAGES) * 2 * ST_K * LD), v0 = k0 + (uint32_t)Cfg::KV;
-    for (int i = threadIdx.x; i < ST_K * CPR; i += THREADS) {
-      const int key = i / CPR, c = i - key * CPR;
-      int page = page_s[(x % ST_PAGES) * ST_K + key];
-      if (page < 0 || page > p.c.n_pages) { atomicOr(p.status, SMC_ERR_BOUNDS); page = 0; }
-      const size_t src = (size_t)page * kv_row + (size_t)kvh * D + c * 8;
-      const uint32_t dst = (uint32_t)(key * LD + c * 8) * 2;
-      st_cp16(k0 + dst, p.k_pool + src);
-      st_cp16(v0 + dst, p.v_pool + src);
-    }
-  };
-  // ids run 2 (STAGES - 1) tiles ahead of the products, keys and values STAGES - 1
-  constexpr int AHEAD = STAGES - 1;
-  static_assert(2 * AHEAD + 1 <= ST_PAGES, "ring of page ids");
-  for (int x = 0; x < AHEAD; ++x) fetch_ids(t_begin + x);
-  asm volatile("cp.async.commit_group;" ::: "memory");
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
-  __syncthreads();
-  for (int x = 0; x < AHEAD; ++x) {
-    fetch(t_begin + x);
-    fetch_ids(t_begin + AHEAD + x);
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
   }
 
+  if constexpr (D == 256) regs_more<ST_MANY>();
+  const int mt = warp % MT, gi = warp / MT, kg = gi & 3, turn = gi >> 2;             // row tile, group; of it keys and turn
+  const float mul = p.c.scale * SH_LOG2E, cap_in = p.c.cap > 0.f ? p.c.scale / p.c.cap : 0.f, cap_out = p.c.cap * SH_LOG2E;
+  bool alive = true;
   int x = t_begin;
   while (x < t_end) {
     // ---------------------------------------------------------------- one sequence's tiles of this worker
@@ -262,31 +315,36 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
     for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
     for (; x < x_end; ++x) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(AHEAD - 1) : "memory");
-      __syncthreads();                                               // tile x has landed, tile x - 1 has been read by everybody
-      fetch(x + AHEAD);
-      fetch_ids(x + 2 * AHEAD);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      const __nv_bfloat16* Kt = kv_s + (size_t)((x - t_begin) % STAGES) * 2 * ST_K * LD + kg * 16 * LD;
+      const int nth = x - t_begin, st = nth % STAGES;
+      if (Cfg::TURNS > 1 && nth % Cfg::TURNS != turn) continue;
+      if (alive) alive = __all_sync(0xffffffffu, st_wait(S, p.status, &S.full[st], (uint32_t)(nth / STAGES) & 1u));
+      if (!alive) continue;
+      const __nv_bfloat16* Kt = kv_s + (size_t)st * 2 * ST_K * LD + kg * 16 * LD;
       const __nv_bfloat16* Vt = Kt + ST_K * LD;
-      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       // matrices of a K fragment: keys 0-7 dims 0-7, keys 0-7 dims 8-15, keys 8-15 dims 0-7, keys 8-15 dims 8-15
       const uint32_t ka = smem_u32(Kt + ((lane & 7) + (lane >> 4) * 8) * LD + ((lane >> 3) & 1) * 8);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        uint32_t b[4];
+      for (int kk = 0; kk < D / 16; kk += 2) {                       // two chains of products
+        uint32_t b[4], d[4];
         st_ldsm(b, ka + kk * 32);
+        st_ldsm(d, ka + kk * 32 + 32);
         st_mma(sc[0], qa[kk], b[0], b[1]);
         st_mma(sc[1], qa[kk], b[2], b[3]);
+        st_mma(sd[0], qa[kk + 1], d[0], d[1]);
+        st_mma(sd[1], qa[kk + 1], d[2], d[3]);
       }
-      const int* pos = pos_s + (x % ST_PAGES) * ST_K + kg * 16;
+      const int i0 = (x - seq0) * ST_K + kg * 16;                    // of the sequence's visible keys
       float top[2] = {m[0], m[1]};
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int kp = pos[n * 8 + 2 * c4 + (i & 1)], r = i >> 1;
-          float v = p.c.cap > 0.f ? shaped_cap(sc[n][i], cap_in, cap_out) : sc[n][i] * mul;
+          const int col = n * 8 + 2 * c4 + (i & 1), r = i >> 1;
+          int kp = p.c.key_pos != nullptr ? pos_s[st * ST_K + kg * 16 + col] : key.begin + i0 + col;
+          kp = i0 + col < key.n ? kp : -1;
+          float v = sc[n][i] + sd[n][i];
+          v = p.c.cap > 0.f ? shaped_cap(v, cap_in, cap_out) : v * mul;
           v = fmaf(slope[r], fabsf((float)(kp - own_pos[r])), v);
           v = kp >= see[r].x && kp <= see[r].y ? v : -INFINITY;
           sc[n][i] = v;
@@ -304,11 +362,16 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
       for (int r = 0; r < 2; ++r) {
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        const float alpha = top[r] == -INFINITY ? 1.f : shaped_ex2(m[r] - top[r]);
-        m[r] = top[r];
-        l[r] *= alpha;
+      }
+      if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) { o[n][2 * r] *= alpha; o[n][2 * r + 1] *= alpha; }
+        for (int r = 0; r < 2; ++r) {
+          const float alpha = top[r] == -INFINITY ? 1.f : shaped_ex2(m[r] - top[r]);
+          m[r] = top[r];
+          l[r] *= alpha;
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) { o[n][2 * r] *= alpha; o[n][2 * r + 1] *= alpha; }
+        }
       }
       float pr[2][4];
 #pragma unroll
@@ -329,30 +392,34 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
         st_mma(o[2 * n], pa, b[0], b[1]);
         st_mma(o[2 * n + 1], pa, b[2], b[3]);
       }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&S.empty[st]);
     }
-    // ---------------------------------------------------------------- the four groups of keys, joined in their order
+    // ---------------------------------------------------------------- the groups of keys, joined one after the other
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
       l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
       if (c4 == 0) {
-        ml_s[kg][mt * 16 + g + 8 * r][0] = m[r];
-        ml_s[kg][mt * 16 + g + 8 * r][1] = l[r];
+        ml_s[gi][mt * 16 + g + 8 * r][0] = m[r];
+        ml_s[gi][mt * 16 + g + 8 * r][1] = l[r];
       }
     }
-    __syncthreads();
+    named_bar(1, THREADS);
     float top[2], sum[2], mine[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int row = mt * 16 + g + 8 * r;
-      top[r] = fmaxf(fmaxf(ml_s[0][row][0], ml_s[1][row][0]), fmaxf(ml_s[2][row][0], ml_s[3][row][0]));
+      top[r] = ml_s[0][row][0];
+#pragma unroll
+      for (int k = 1; k < Cfg::GROUPS; ++k) top[r] = fmaxf(top[r], ml_s[k][row][0]);
       sum[r] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum[r] += top[r] == -INFINITY ? 0.f : ml_s[k][row][1] * shaped_ex2(ml_s[k][row][0] - top[r]);
+      for (int k = 0; k < Cfg::GROUPS; ++k) sum[r] += top[r] == -INFINITY ? 0.f : ml_s[k][row][1] * shaped_ex2(ml_s[k][row][0] - top[r]);
       mine[r] = top[r] == -INFINITY ? 0.f : shaped_ex2(m[r] - top[r]);
     }
-    for (int k = 0; k < 4; ++k) {
-      if (kg == k) {
+    for (int k = 0; k < Cfg::GROUPS; ++k) {
+      if (gi == k) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           float* at = join + (mt * 16 + g + 8 * r) * (D + 4);
@@ -363,10 +430,10 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
             // a row that no key of this group is visible to adds nothing, whatever its values are
             *cell = mine[r] == 0.f ? before : make_float2(before.x + o[n][2 * r] * mine[r], before.y + o[n][2 * r + 1] * mine[r]);
           }
-          if (k == 3 && c4 == 0) { at[D] = top[r]; at[D + 1] = sum[r]; }
+          if (k == Cfg::GROUPS - 1 && c4 == 0) { at[D] = top[r]; at[D + 1] = sum[r]; }
         }
       }
-      __syncthreads();
+      named_bar(1, THREADS);
     }
     const int w_first = step_owner(seq0, W, total), w_last = step_owner(seq1 - 1, W, total), R = M - m0;
     bool finish = w_first == w_last;
@@ -378,15 +445,15 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
       float* to = part(w);
       for (int i = threadIdx.x; i < R * (D + 2); i += THREADS) to[i] = join[i / (D + 2) * (D + 4) + i % (D + 2)];
       __threadfence();
-      __syncthreads();
+      named_bar(1, THREADS);
       if (threadIdx.x == 0) {
         const int n = w_last - w_first + 1;
-        last_s = atomicAdd(counter + s * p.Hkv, 1) == n - 1;
-        if (last_s) counter[s * p.Hkv] = 0;
+        S.last = atomicAdd(counter + s * p.Hkv, 1) == n - 1;
+        if (S.last) counter[s * p.Hkv] = 0;
         __threadfence();
       }
-      __syncthreads();
-      finish = last_s != 0;
+      named_bar(1, THREADS);
+      finish = S.last != 0;
       if (finish) {                                                  // all parts are there
         for (int r = warp; r < R; r += Cfg::WARPS) {                 // a warp per row
           float big = -INFINITY;
@@ -407,7 +474,7 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
           for (int n = 0; n < D / 32; ++n) at[n * 32 + lane] = acc[n];
           if (lane == 0) { at[D] = big; at[D + 1] = den; }
         }
-        __syncthreads();
+        named_bar(1, THREADS);
       }
     }
     if (finish) {
@@ -430,9 +497,8 @@ __global__ void __launch_bounds__(StCfg<D, MT>::WARPS * 32, MT == 1 && D <= 128 
           if (p.scores != nullptr) p.lse2[to] = none ? INFINITY : v;
         }
     }
-    __syncthreads();                                                 // `join` is free for the next sequence
+    named_bar(1, THREADS);                                                 // `join` is free for the next sequence
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // mass[row, kvh, j] += sum over the rows of exp2(score - lse)
@@ -473,13 +539,13 @@ __global__ void __launch_bounds__(256) shaped_step_mass_kernel(const ShapedStepP
 // Parts of the workspace, each from a 256-byte border.
 struct StepWork { size_t parts, lse2, scores, bytes; long long score_tiles, counted; int workers; };
 
-// Row tiles of a CTA: its registers hold 16 rows of outputs a warp, D = 256 has room for two of them (more rows: further CTAs).
-static int step_row_tiles(int M, int D) { return M <= 16 ? 1 : M <= 32 || D == 256 ? 2 : 4; }
+// Row tiles of a CTA: a warp's registers hold 16 rows of outputs; more than 32 rows go to further CTAs, which find the keys in L2.
+static int step_row_tiles(int M) { return M <= 16 ? 1 : 2; }
 
 static StepWork step_work(int bs, int E, int Hq, int Hkv, int D, long long keys) {
   StepWork w;
-  const int M = E * (Hq / Hkv), mt = step_row_tiles(M, D), blocks = (M + 16 * mt - 1) / (16 * mt), per_sm = mt == 1 && D <= 128 ? 2 : 1;
-  w.workers = (148 * per_sm + Hkv * blocks - 1) / (Hkv * blocks);
+  const int M = E * (Hq / Hkv), mt = step_row_tiles(M), blocks = (M + 16 * mt - 1) / (16 * mt);
+  w.workers = 148 / (Hkv * blocks) > 0 ? 148 / (Hkv * blocks) : 1;  // a CTA per SM
   w.score_tiles = keys > 0 ? keys / ST_K + bs : 0;                   // every sequence may end inside a tile
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   w.counted = (long long)bs * Hkv * blocks;
@@ -493,14 +559,18 @@ static StepWork step_work(int bs, int E, int Hq, int Hkv, int D, long long keys)
 template <int D, int MT>
 static int launch_shaped_step(const ShapedStepParams& p, cudaStream_t st) {
   using Cfg = StCfg<D, MT>;
-  static_assert(Cfg::SMEM + 4 * 16 * MT * 8 + 64 <= 232448, "shared memory");
+  static_assert(Cfg::SMEM + Cfg::GROUPS * 16 * MT * 8 + sizeof(StShared) <= 232448, "shared memory");
   CUDA_CHECK_RET(cudaFuncSetAttribute(shaped_step_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::SMEM));
+  if constexpr (D == 256) {                           // what the warps ask for later is there from the start
+    static const int regs = [] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, shaped_step_kernel<D, MT>) == cudaSuccess ? a.numRegs : 0; }();
+    if (regs < 168) return -155;
+  }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)p.workers, (unsigned)p.Hkv, (unsigned)((p.E * (p.Hq / p.Hkv) + 16 * MT - 1) / (16 * MT)));
-  cfg.blockDim = dim3(Cfg::WARPS * 32);
+  cfg.blockDim = dim3(Cfg::THREADS);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = st;
   cfg.attrs = attr;
@@ -525,12 +595,12 @@ SMC_API long long smc_shaped_step_work(int bs, int E, int Hq, int Hkv, int D, lo
 }
 
 // q, out: bs * E rows of Hq * D bf16 values, the E tokens of a sequence are the last of its lens[s] cached ones (rows [bs], lens [bs] int32).
-// work: zeros at first, smc_shaped_step_work bytes of `keys`.  mass [bt_rows, Hkv, mass_stride] fp32 or null.
+// work: zeros at first, smc_shaped_step_work bytes or more; with the mass it has to hold the scores of all cached tokens of the batch.  mass [bt_rows, Hkv, mass_stride] fp32 or null.
 SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, const void* v_pool, int n_pages, const int* block_table,
                             int bt_stride, int bt_rows, const int* key_pos, int kp_stride, const int* rows, const int* lens, void* out,
                             long long ld_out, float* lse, float* mass, long long mass_stride, int bs, int E, int Hq, int Hkv, int D,
                             float scale, float cap, const float* slopes, const int* bounds, void* work, long long work_bytes,
-                            long long keys, int* status, int pdl, cudaStream_t st) {
+                            int* status, int pdl, cudaStream_t st) {
   using namespace smc;
   if (bs <= 0) return 0;
   if (smc_shaped_step_work(bs, E, Hq, Hkv, D, 0) < 0) return -150;
@@ -539,9 +609,10 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -151;
   if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -152;
-  if (mass != nullptr && (keys <= 0 || mass_stride < bt_stride)) return -153;
-  const StepWork w = step_work(bs, E, Hq, Hkv, D, mass != nullptr ? keys : 0);
-  if (work_bytes < (long long)w.bytes) return -154;
+  if (mass != nullptr && mass_stride < bt_stride) return -153;
+  StepWork w = step_work(bs, E, Hq, Hkv, D, 0);
+  if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hq * E * ST_K * 4);       // the rest of it
+  if (work_bytes < (long long)w.bytes || (mass != nullptr && w.score_tiles < 1)) return -154;
   ShapedStepParams p;
   p.c = ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, scale, cap};
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.v_pool = (const __nv_bfloat16*)v_pool;
@@ -551,12 +622,11 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
   p.scores = mass != nullptr ? (float*)(base + w.scores) : nullptr;
   p.ld_q = ld_q; p.ld_out = ld_out; p.mass_stride = mass_stride; p.score_tiles = w.score_tiles;
   p.bs = bs; p.E = E; p.Hq = Hq; p.Hkv = Hkv; p.workers = w.workers; p.pdl = pdl; p.status = status;
-  const int mt = step_row_tiles(E * (Hq / Hkv), D);
+  const int mt = step_row_tiles(E * (Hq / Hkv));
 #define SMC_SHAPED_STEP(DD)                                      \
   if (D == DD) {                                                 \
     if (mt == 1) return launch_shaped_step<DD, 1>(p, st);        \
-    if (mt == 2) return launch_shaped_step<DD, 2>(p, st);        \
-    if constexpr (DD != 256) return launch_shaped_step<DD, 4>(p, st); \
+    return launch_shaped_step<DD, 2>(p, st);                     \
   }
   SMC_SHAPED_STEP(64)
   SMC_SHAPED_STEP(128)

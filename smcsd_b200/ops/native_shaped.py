@@ -37,7 +37,7 @@ def _library():
     if _lib is None:
         L, vp, i, ll, f = K.lib(), C.c_void_p, C.c_int, C.c_longlong, C.c_float
         L.smc_shaped_prompt.argtypes = [vp, ll, vp, vp, i, vp, i, i, vp, i, vp, i, vp, ll, vp, i, i, i, i, f, f, vp, vp, vp, i, vp]
-        L.smc_shaped_step.argtypes = [vp, ll, vp, vp, i, vp, i, i, vp, i, vp, vp, vp, ll, vp, vp, ll, i, i, i, i, i, f, f, vp, vp, vp, ll, ll, vp, i, vp]
+        L.smc_shaped_step.argtypes = [vp, ll, vp, vp, i, vp, i, i, vp, i, vp, vp, vp, ll, vp, vp, ll, i, i, i, i, i, f, f, vp, vp, vp, ll, vp, i, vp]
         L.smc_shaped_mass.argtypes = [vp, ll, vp, i, vp, i, i, vp, i, vp, i, vp, vp, ll, i, i, i, i, f, f, vp, vp, vp, i, vp]
         L.smc_evict.argtypes = [vp, ll, vp, ll, vp, ll, vp, i, vp, vp, i, i, i, i, i, vp, vp, vp, vp, i, vp, ll, vp, vp]
         L.smc_shaped_step_work.argtypes = [i, i, i, i, i, ll]
@@ -173,14 +173,11 @@ def attention_shaped_step(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     kp, kps = _table(key_pos, "key_pos", dev, block_table.shape[0], block_table.shape[1])
     sl, bo, st = _shape(dev, T, Hq, slopes, bounds, status)
     mp, ms = (None, 0) if mass is None else _weights(mass, dev, block_table.shape[0], Hkv, block_table.shape[1])
-    nbytes, keys = work.numel(), 0
-    if mass is not None:                                             # as many keys as the workspace has room for
-        fixed = shaped_step_work_bytes(bs, E, Hq, Hkv, D) + 256
-        keys = ((nbytes - fixed) // (Hq * E * 256) - bs) * 64 + 63
     K._check(L.smc_shaped_step(qp, ldq, _pool(k_pool, "k_pool", dev, Hkv * D), _pool(v_pool, "v_pool", dev, Hkv * D), min(k_pool.shape[0], v_pool.shape[0]) - 1, bt,
                                block_table.shape[1] if block_table.shape[0] == 1 else bts, block_table.shape[0], kp, kps, _is(rows, "rows", _I32, dev, (bs,)),
                                _is(lens, "lens", _I32, dev, (bs,)), op, ldo, None if lse is None else _is(lse, "lse", _F32, dev, (T, Hq)), mp, ms, bs, E, Hq, Hkv, D,
-                               scale, softcap, sl, bo, _is(work, "work", _U8, dev, work.shape), nbytes, keys, st, int(pdl), K._stream()), "smc_shaped_step")
+                               scale, softcap, sl, bo, _is(work, "work", _U8, dev, work.shape), work.numel(), st, int(pdl), K._stream()),
+             "smc_shaped_step")
 
 
 def evict_work_bytes(n_pages: int) -> int:
