@@ -3,9 +3,14 @@
 //
 // What bounds it is the cache: 4 D bytes per key and KV head, read once.  The keys of all sequences, cut into tiles of 64, are one line of
 // work per KV head that W workers share in equal parts, wherever sequences begin and end: a batch of ragged contexts keeps every SM busy to the
-// end, and a single sequence is spread over all of them.  A CTA gathers its tiles page by page with cp.async, three of them in flight, and
-// its warps take 16 keys each (mma.sync: a tile of a dozen rows is short against the gather, and the tensor memory's 128 lanes would stay
-// empty).  Where a sequence ends inside a worker's part its state goes to the workspace, and the worker that comes last joins the
+// end, and a single sequence is spread over all of them.  Four loader warps gather the tiles page by page with cp.async into a ring; the other
+// warps take 16 keys each, two tiles in turn, and come to the loaders' ring only through its barriers.
+//
+// Keys are the rows of the products (mma.sync, 16 x 8 x 16) and queries their eight columns: S^T = K Q^T and O^T += V^T P^T, so that the
+// four or eight heads of a group fill a fragment (as rows of sixteen they left half of every product and of the softmax idle: a tile of D = 64 took 1000 cycles of an SM
+// instead of the 700 its bytes take).  tcgen05 has no such narrow form: its 128 lanes would hold keys, and the softmax would run across lanes.
+//
+// Where a sequence ends inside a worker's part its state goes to the workspace, and the worker that comes last joins the
 // parts of a (sequence, KV head) in the order of its keys, so that results do not depend on the order of arrival.
 //
 // With ``mass`` the scores of all (row, key) pairs stay in the workspace (4 E G bytes per key and KV head, against 4 D of the cache), and a second
@@ -32,9 +37,9 @@ struct ShapedStepParams {
   float* mass;                   // [bt_rows, Hkv, mass_stride] or null
   // workspace
   int* counters;                 // [row blocks][bs][Hkv], zero between calls
-  float* parts;                  // [W][2][Hkv][E G][D + 2]
+  float* parts;                  // [W][2][Hkv][E G][D + 4]
   float* lse2;                   // [bs * E, Hq] in base 2, +inf where nothing is visible
-  float* scores;                 // [Hkv][score_tiles][E G][64]
+  float* scores;                 // [Hkv][score_tiles][64][pitch], pitch E G rounded up to 4
   long long ld_q, ld_out, mass_stride, score_tiles;
   int bs, E, Hq, Hkv, workers, pdl;
   int* status;
@@ -94,6 +99,12 @@ __device__ __forceinline__ void st_ldsm(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void st_ldsm_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// an 8 x 8 matrix of bf16 values, two neighbours of a row per lane, transposed
+__device__ __forceinline__ uint32_t st_transpose(uint32_t v) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(v));
+  return y;
+}
 __device__ __forceinline__ uint32_t st_pack(float a, float b) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
@@ -136,15 +147,19 @@ __device__ __forceinline__ int step_sequence(const int* tiles, int bs, int x) {
   return lo;
 }
 
-template <int D, int MT>
+// A warp takes NQ columns of eight rows, MT warps side by side all rows of the CTA.
+template <int D, int NQ, int MT>
 struct StCfg {
-  // consumers: row tiles of 16 x four groups of 16 keys, twice (tiles in turn) where that makes eight warps
-  static constexpr int TURNS = MT == 1 ? 2 : 1, GROUPS = 4 * TURNS, WARPS = GROUPS * MT, THREADS = (WARPS + ST_LOADERS) * 32;
+  static constexpr int ROWS = 8 * NQ * MT;
+  // groups of keys in a tile, tiles in turn: eight consumer warps; four with D = 256, whose 16 keys a warp holds while it works are 16 KB
+  static constexpr int GW = MT == 4 ? 2 : 4, SUB = 4 / GW, TURNS = MT == 1 && D < 256 ? 2 : 1;
+  static constexpr int GROUPS = GW * TURNS, WARPS = GROUPS * MT, THREADS = (WARPS + ST_LOADERS) * 32;
   static constexpr int LD = D + 8;
   static constexpr int STAGES = D == 64 ? 8 : D == 128 ? 5 : MT == 1 ? 3 : 2;
+  static constexpr int SLOTS = D == 256 ? (ROWS == 8 ? 2 : 1) : 64 / ROWS;           // states that groups leave at once when they are joined
   static constexpr size_t KV = (size_t)ST_K * LD * 2;                // one of K, V
-  // stages, a state of [16 MT][D + 4] for the join, positions of the tiles in flight, prefix sums
-  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)16 * MT * (D + 4) * 4 + (size_t)STAGES * ST_K * 4 + (ST_MAX_BS + 1 + 64) * 4;
+  // stages, states, positions of the tiles in flight, prefix sums
+  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)SLOTS * ROWS * (D + 4) * 4 + (size_t)STAGES * ST_K * 4 + (ST_MAX_BS + 1 + 64) * 4;
 };
 
 // A place in the line of tiles: the sequence that tile x belongs to.
@@ -180,43 +195,45 @@ __device__ __forceinline__ bool st_wait(StShared& S, int* status, uint64_t* bar,
   }
 }
 
-template <int D, int MT>
-__global__ void __launch_bounds__(StCfg<D, MT>::THREADS, 1) shaped_step_kernel(const ShapedStepParams p) {
-  using Cfg = StCfg<D, MT>;
+template <int D, int NQ, int MT>
+__global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kernel(const ShapedStepParams p) {
+  using Cfg = StCfg<D, NQ, MT>;
   constexpr int LD = Cfg::LD, STAGES = Cfg::STAGES, THREADS = Cfg::WARPS * 32, CPR = D / 8;
   extern __shared__ __align__(128) uint8_t st_smem[];
   __nv_bfloat16* kv_s = reinterpret_cast<__nv_bfloat16*>(st_smem);   // [stage][K, V][64][LD]
-  float* join = reinterpret_cast<float*>(st_smem + STAGES * 2 * Cfg::KV);            // [16 MT][D + 4]
-  int* pos_s = reinterpret_cast<int*>(join + 16 * MT * (D + 4));     // [stage][64]
+  float* join = reinterpret_cast<float*>(st_smem + STAGES * 2 * Cfg::KV);            // [slot][ROWS][D + 4]
+  int* pos_s = reinterpret_cast<int*>(join + Cfg::SLOTS * Cfg::ROWS * (D + 4));      // [stage][64]
   int* tiles = pos_s + STAGES * ST_K;                                // [bs + 1]
   int* misc = tiles + ST_MAX_BS + 1;                                 // [64]
-  __shared__ float ml_s[Cfg::GROUPS][16 * MT][2];
+  __shared__ float ml_s[Cfg::GROUPS][Cfg::ROWS][2];
+  __shared__ float4 row_s[Cfg::ROWS];                                // of a row: first and last visible position, its own, slope
   __shared__ StShared S;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c4 = lane & 3;
-  // rows r = token * G + head of this CTA: [m0, M)
-  const int G = p.Hq / p.Hkv, m0 = blockIdx.z * 16 * MT, rows_all = p.E * G, M = min(rows_all, m0 + 16 * MT), kvh = blockIdx.y, w = blockIdx.x;
-  int* counter = p.counters + ((size_t)blockIdx.z * p.bs) * p.Hkv + kvh;
+  const int G = p.Hq / p.Hkv, M = p.E * G, kvh = blockIdx.y, w = blockIdx.x;         // rows r = token * G + head
+  int* counter = p.counters + kvh;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&S.full[i], ST_LOADERS * 32);
-      mbar_init(&S.empty[i], 4 * MT);
+      mbar_init(&S.empty[i], Cfg::GW * MT);
     }
     S.abort = 0;
     fence_barrier_init();
   }
-  if (p.pdl) { pdl_launch_dependents(); pdl_wait_prior_grid(); }
+  // a mass kernel behind this one reads rows and lengths ahead of its wait: they have to be there before it may start
+  if (p.pdl) pdl_wait_prior_grid();
+  pdl_launch_dependents();
   step_schedule(p, tiles, misc);
   const int total = tiles[p.bs];
   // sequences without a tile have nobody else to write their rows
   if (w == 0) {
     for (int s = warp; s < p.bs; s += Cfg::THREADS / 32) {
       if (tiles[s + 1] > tiles[s]) continue;
-      for (int x = m0 * D + lane; x < M * D; x += 32) {
+      for (int x = lane; x < M * D; x += 32) {
         const int e = x / (G * D), hd = x - e * G * D;
         p.out[(size_t)(s * p.E + e) * p.ld_out + (size_t)kvh * G * D + hd] = __float2bfloat16(0.f);
       }
-      for (int x = m0 + lane; x < M; x += 32) {
+      for (int x = lane; x < M; x += 32) {
         const size_t at = (size_t)(s * p.E + x / G) * p.Hq + kvh * G + x % G;
         if (p.lse != nullptr) p.lse[at] = -INFINITY;
         if (p.scores != nullptr) p.lse2[at] = INFINITY;
@@ -228,7 +245,7 @@ __global__ void __launch_bounds__(StCfg<D, MT>::THREADS, 1) shaped_step_kernel(c
   const int t_begin = step_first(w, W, total), t_end = step_first(w + 1, W, total);
 
   if (warp >= Cfg::WARPS) {
-    if constexpr (D == 256) regs_fewer<ST_FEW>();
+    if constexpr (D == 256 && Cfg::THREADS == 384) regs_fewer<ST_FEW>();
     // ================================================================= loaders: 16 keys of each tile a warp
     const int lw = warp - Cfg::WARPS, kl0 = lw * 16 + (lane & 15);
     const size_t kv_row = (size_t)p.Hkv * D;
@@ -273,177 +290,213 @@ __global__ void __launch_bounds__(StCfg<D, MT>::THREADS, 1) shaped_step_kernel(c
     return;
   }
 
-  if constexpr (D == 256) regs_more<ST_MANY>();
-  const int mt = warp % MT, gi = warp / MT, kg = gi & 3, turn = gi >> 2;             // row tile, group; of it keys and turn
+  if constexpr (D == 256 && Cfg::THREADS == 384) regs_more<ST_MANY>();
+  const int mt = warp % MT, gi = warp / MT, kg = gi % Cfg::GW, turn = gi / Cfg::GW;  // row set, group; of it keys and turn
   const float mul = p.c.scale * SH_LOG2E, cap_in = p.c.cap > 0.f ? p.c.scale / p.c.cap : 0.f, cap_out = p.c.cap * SH_LOG2E;
+  const int pitch = (M + 3) / 4 * 4;
   bool alive = true;
   int x = t_begin;
   while (x < t_end) {
     // ---------------------------------------------------------------- one sequence's tiles of this worker
     const int s = step_sequence(tiles, p.bs, x), seq0 = tiles[s], seq1 = tiles[s + 1], x_end = min(t_end, seq1);
     const StepKeys key = step_keys(p, s);
-    uint32_t qa[D / 16][4];
-    {
-      const int r0 = m0 + mt * 16 + g, r1 = r0 + 8;
-      const __nv_bfloat16* q0 = p.q + (size_t)(s * p.E + r0 / G) * p.ld_q + (size_t)(kvh * G + r0 % G) * D + 2 * c4;
-      const __nv_bfloat16* q1 = p.q + (size_t)(s * p.E + r1 / G) * p.ld_q + (size_t)(kvh * G + r1 % G) * D + 2 * c4;
+    for (int r = threadIdx.x; r < Cfg::ROWS; r += THREADS) {
+      const int idx = key.len - p.E + r / G;
+      float4 v = make_float4((float)SH_POS_END, -1.f, 0.f, 0.f);
+      if (r < M && idx >= 0) {
+        const int pos = p.c.key_pos != nullptr ? p.c.key_pos[(size_t)key.row * p.c.kp_stride + idx] : idx;
+        const int2 see = shaped_bounds(p.c, s * p.E + r / G, pos);
+        v = make_float4((float)see.x, (float)see.y, (float)pos, p.c.slopes != nullptr ? -p.c.slopes[kvh * G + r % G] * SH_LOG2E : 0.f);
+      }
+      row_s[r] = v;
+    }
+    uint32_t qb[NQ][D / 16][2];                                      // Q^T fragments: row g of each column set
+#pragma unroll
+    for (int q = 0; q < NQ; ++q) {
+      const int r = (mt * NQ + q) * 8 + g;
+      const __nv_bfloat16* q0 = p.q + (size_t)(s * p.E + r / G) * p.ld_q + (size_t)(kvh * G + r % G) * D + 2 * c4;
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk) {
-        qa[kk][0] = r0 < M ? *reinterpret_cast<const uint32_t*>(q0 + kk * 16) : 0u;
-        qa[kk][1] = r1 < M ? *reinterpret_cast<const uint32_t*>(q1 + kk * 16) : 0u;
-        qa[kk][2] = r0 < M ? *reinterpret_cast<const uint32_t*>(q0 + kk * 16 + 8) : 0u;
-        qa[kk][3] = r1 < M ? *reinterpret_cast<const uint32_t*>(q1 + kk * 16 + 8) : 0u;
+        qb[q][kk][0] = r < M ? *reinterpret_cast<const uint32_t*>(q0 + kk * 16) : 0u;
+        qb[q][kk][1] = r < M ? *reinterpret_cast<const uint32_t*>(q0 + kk * 16 + 8) : 0u;
       }
     }
-    int2 see[2];
-    int own_pos[2];
-    float slope[2];
+    named_bar(1, THREADS);                                           // rows are known
+    float m[NQ][2], l[NQ][2], o[NQ][D / 16][4];                      // of columns 2 c4, 2 c4 + 1
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = m0 + mt * 16 + g + 8 * i, e = r / G, idx = key.len - p.E + e;
-      own_pos[i] = 0;
-      see[i] = make_int2(SH_POS_END, -1);
-      slope[i] = 0.f;
-      if (r < M && idx >= 0) {
-        own_pos[i] = p.c.key_pos != nullptr ? p.c.key_pos[(size_t)key.row * p.c.kp_stride + idx] : idx;
-        see[i] = shaped_bounds(p.c, s * p.E + e, own_pos[i]);
-        if (p.c.slopes != nullptr) slope[i] = -p.c.slopes[kvh * G + r % G] * SH_LOG2E;
-      }
+    for (int q = 0; q < NQ; ++q) {
+      m[q][0] = m[q][1] = -INFINITY;
+      l[q][0] = l[q][1] = 0.f;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) o[q][n][0] = o[q][n][1] = o[q][n][2] = o[q][n][3] = 0.f;
     }
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
     for (; x < x_end; ++x) {
       const int nth = x - t_begin, st = nth % STAGES;
       if (Cfg::TURNS > 1 && nth % Cfg::TURNS != turn) continue;
       if (alive) alive = __all_sync(0xffffffffu, st_wait(S, p.status, &S.full[st], (uint32_t)(nth / STAGES) & 1u));
       if (!alive) continue;
-      const __nv_bfloat16* Kt = kv_s + (size_t)st * 2 * ST_K * LD + kg * 16 * LD;
-      const __nv_bfloat16* Vt = Kt + ST_K * LD;
-      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}}, sd[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      // matrices of a K fragment: keys 0-7 dims 0-7, keys 0-7 dims 8-15, keys 8-15 dims 0-7, keys 8-15 dims 8-15
-      const uint32_t ka = smem_u32(Kt + ((lane & 7) + (lane >> 4) * 8) * LD + ((lane >> 3) & 1) * 8);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; kk += 2) {                       // two chains of products
-        uint32_t b[4], d[4];
-        st_ldsm(b, ka + kk * 32);
-        st_ldsm(d, ka + kk * 32 + 32);
-        st_mma(sc[0], qa[kk], b[0], b[1]);
-        st_mma(sc[1], qa[kk], b[2], b[3]);
-        st_mma(sd[0], qa[kk + 1], d[0], d[1]);
-        st_mma(sd[1], qa[kk + 1], d[2], d[3]);
-      }
-      const int i0 = (x - seq0) * ST_K + kg * 16;                    // of the sequence's visible keys
-      float top[2] = {m[0], m[1]};
+      for (int sub = 0; sub < Cfg::SUB; ++sub) {
+        const int k0 = (kg * Cfg::SUB + sub) * 16;
+        const __nv_bfloat16* Kt = kv_s + (size_t)st * 2 * ST_K * LD + k0 * LD;
+        const __nv_bfloat16* Vt = Kt + ST_K * LD;
+        float sc[NQ][4], sd[NQ][4];                                  // two chains of products
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int q = 0; q < NQ; ++q) sc[q][0] = sc[q][1] = sc[q][2] = sc[q][3] = sd[q][0] = sd[q][1] = sd[q][2] = sd[q][3] = 0.f;
+        // matrices of a K fragment: keys 0-7 dims 0-7, keys 8-15 dims 0-7, keys 0-7 dims 8-15, keys 8-15 dims 8-15
+        const uint32_t ka = smem_u32(Kt + (lane & 15) * LD + (lane >> 4) * 8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int col = n * 8 + 2 * c4 + (i & 1), r = i >> 1;
-          int kp = p.c.key_pos != nullptr ? pos_s[st * ST_K + kg * 16 + col] : key.begin + i0 + col;
-          kp = i0 + col < key.n ? kp : -1;
-          float v = sc[n][i] + sd[n][i];
-          v = p.c.cap > 0.f ? shaped_cap(v, cap_in, cap_out) : v * mul;
-          v = fmaf(slope[r], fabsf((float)(kp - own_pos[r])), v);
-          v = kp >= see[r].x && kp <= see[r].y ? v : -INFINITY;
-          sc[n][i] = v;
-          top[r] = fmaxf(top[r], v);
+        for (int kk = 0; kk < D / 16; kk += 2) {
+          uint32_t a[4], b[4];
+          st_ldsm(a, ka + kk * 32);
+          st_ldsm(b, ka + kk * 32 + 32);
+#pragma unroll
+          for (int q = 0; q < NQ; ++q) {
+            st_mma(sc[q], a, qb[q][kk][0], qb[q][kk][1]);
+            st_mma(sd[q], b, qb[q][kk + 1][0], qb[q][kk + 1][1]);
+          }
         }
-      if (p.scores != nullptr && x < p.score_tiles) {
-        float* at = p.scores + (((size_t)kvh * p.score_tiles + x) * rows_all + m0 + mt * 16 + g) * ST_K + kg * 16 + 2 * c4;
+        const int i0 = (x - seq0) * ST_K + k0 + g;                   // of the sequence's visible keys: this lane's, and the one 8 behind
+        float kp[2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          if (m0 + mt * 16 + g < M) *reinterpret_cast<float2*>(at + n * 8) = make_float2(sc[n][0], sc[n][1]);
-          if (m0 + mt * 16 + g + 8 < M) *reinterpret_cast<float2*>(at + 8 * ST_K + n * 8) = make_float2(sc[n][2], sc[n][3]);
+        for (int h = 0; h < 2; ++h) {
+          const int pos = p.c.key_pos != nullptr ? pos_s[st * ST_K + k0 + g + 8 * h] : key.begin + i0 + 8 * h;
+          kp[h] = i0 + 8 * h < key.n ? (float)pos : -1.f;
         }
-      }
+        uint32_t pb[NQ][2];
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      }
-      if (__any_sync(0xffffffffu, top[0] > m[0] || top[1] > m[1])) {
+        for (int q = 0; q < NQ; ++q) {
+          float top[2] = {m[q][0], m[q][1]};
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float alpha = top[r] == -INFINITY ? 1.f : shaped_ex2(m[r] - top[r]);
-          m[r] = top[r];
-          l[r] *= alpha;
+          for (int i = 0; i < 4; ++i) {
+            const float4 row = row_s[(mt * NQ + q) * 8 + 2 * c4 + (i & 1)];
+            float v = sc[q][i] + sd[q][i];
+            v = p.c.cap > 0.f ? shaped_cap(v, cap_in, cap_out) : v * mul;
+            v = fmaf(row.w, fabsf(kp[i >> 1] - row.z), v);
+            v = kp[i >> 1] >= row.x && kp[i >> 1] <= row.y ? v : -INFINITY;
+            sc[q][i] = v;
+            top[i & 1] = fmaxf(top[i & 1], v);
+          }
+          if (p.scores != nullptr && x < p.score_tiles) {
+            const int r = (mt * NQ + q) * 8 + 2 * c4;
+            float* at = p.scores + (((size_t)kvh * p.score_tiles + x) * ST_K + k0 + g) * pitch + r;
+            if (r < pitch) {
+              *reinterpret_cast<float2*>(at) = make_float2(sc[q][0], sc[q][1]);
+              *reinterpret_cast<float2*>(at + 8 * pitch) = make_float2(sc[q][2], sc[q][3]);
+            }
+          }
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) { o[n][2 * r] *= alpha; o[n][2 * r + 1] *= alpha; }
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int sh = 4; sh < 32; sh <<= 1) top[c] = fmaxf(top[c], __shfl_xor_sync(0xffffffffu, top[c], sh));
+          if (__any_sync(0xffffffffu, top[0] > m[q][0] || top[1] > m[q][1])) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              const float alpha = top[c] == -INFINITY ? 1.f : shaped_ex2(m[q][c] - top[c]);
+              m[q][c] = top[c];
+              l[q][c] *= alpha;
+#pragma unroll
+              for (int n = 0; n < D / 16; ++n) { o[q][n][c] *= alpha; o[q][n][2 + c] *= alpha; }
+            }
+          }
+          const float ref[2] = {m[q][0] == -INFINITY ? 0.f : m[q][0], m[q][1] == -INFINITY ? 0.f : m[q][1]};
+          float pr[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            pr[i] = shaped_ex2(sc[q][i] - ref[i & 1]);
+            l[q][i & 1] += pr[i];
+          }
+          pb[q][0] = st_transpose(st_pack(pr[0], pr[1]));
+          pb[q][1] = st_transpose(st_pack(pr[2], pr[3]));
         }
-      }
-      float pr[2][4];
+        // matrices of a V^T fragment: dims 0-7 keys 0-7, dims 8-15 keys 0-7, dims 0-7 keys 8-15, dims 8-15 keys 8-15
+        const uint32_t va = smem_u32(Vt + ((lane & 7) + (lane >> 4) * 8) * LD + ((lane >> 3) & 1) * 8);
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < D / 16; ++n) {
+          uint32_t a[4];
+          st_ldsm_t(a, va + n * 32);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = i >> 1;
-          pr[n][i] = m[r] == -INFINITY ? 0.f : shaped_ex2(sc[n][i] - m[r]);
-          l[r] += pr[n][i];
+          for (int q = 0; q < NQ; ++q) st_mma(o[q][n], a, pb[q][0], pb[q][1]);
         }
-      const uint32_t pa[4] = {st_pack(pr[0][0], pr[0][1]), st_pack(pr[0][2], pr[0][3]), st_pack(pr[1][0], pr[1][1]), st_pack(pr[1][2], pr[1][3])};
-      // matrices of a V fragment: keys 0-7 dims 0-7, keys 8-15 dims 0-7, keys 0-7 dims 8-15, keys 8-15 dims 8-15
-      const uint32_t va = smem_u32(Vt + (lane & 15) * LD + (lane >> 4) * 8);
-#pragma unroll
-      for (int n = 0; n < D / 16; ++n) {
-        uint32_t b[4];
-        st_ldsm_t(b, va + n * 32);
-        st_mma(o[2 * n], pa, b[0], b[1]);
-        st_mma(o[2 * n + 1], pa, b[2], b[3]);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&S.empty[st]);
     }
-    // ---------------------------------------------------------------- the groups of keys, joined one after the other
+    // ---------------------------------------------------------------- the groups of keys, joined in their order
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (c4 == 0) {
-        ml_s[gi][mt * 16 + g + 8 * r][0] = m[r];
-        ml_s[gi][mt * 16 + g + 8 * r][1] = l[r];
-      }
-    }
-    named_bar(1, THREADS);
-    float top[2], sum[2], mine[2];
+    for (int q = 0; q < NQ; ++q)
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = mt * 16 + g + 8 * r;
-      top[r] = ml_s[0][row][0];
+      for (int c = 0; c < 2; ++c) {
 #pragma unroll
-      for (int k = 1; k < Cfg::GROUPS; ++k) top[r] = fmaxf(top[r], ml_s[k][row][0]);
-      sum[r] = 0.f;
-#pragma unroll
-      for (int k = 0; k < Cfg::GROUPS; ++k) sum[r] += top[r] == -INFINITY ? 0.f : ml_s[k][row][1] * shaped_ex2(ml_s[k][row][0] - top[r]);
-      mine[r] = top[r] == -INFINITY ? 0.f : shaped_ex2(m[r] - top[r]);
-    }
-    for (int k = 0; k < Cfg::GROUPS; ++k) {
-      if (gi == k) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float* at = join + (mt * 16 + g + 8 * r) * (D + 4);
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n) {
-            float2* cell = reinterpret_cast<float2*>(at + n * 8 + 2 * c4);
-            const float2 before = k == 0 ? make_float2(0.f, 0.f) : *cell;
-            // a row that no key of this group is visible to adds nothing, whatever its values are
-            *cell = mine[r] == 0.f ? before : make_float2(before.x + o[n][2 * r] * mine[r], before.y + o[n][2 * r + 1] * mine[r]);
-          }
-          if (k == Cfg::GROUPS - 1 && c4 == 0) { at[D] = top[r]; at[D + 1] = sum[r]; }
+        for (int sh = 4; sh < 32; sh <<= 1) l[q][c] += __shfl_xor_sync(0xffffffffu, l[q][c], sh);
+        if (g == 0) {
+          ml_s[gi][(mt * NQ + q) * 8 + 2 * c4 + c][0] = m[q][c];
+          ml_s[gi][(mt * NQ + q) * 8 + 2 * c4 + c][1] = l[q][c];
         }
+      }
+    named_bar(1, THREADS);
+    float mine[NQ][2];
+#pragma unroll
+    for (int q = 0; q < NQ; ++q)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int row = (mt * NQ + q) * 8 + 2 * c4 + c;
+        float top = ml_s[0][row][0];
+#pragma unroll
+        for (int k = 1; k < Cfg::GROUPS; ++k) top = fmaxf(top, ml_s[k][row][0]);
+        float sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < Cfg::GROUPS; ++k) sum += top == -INFINITY ? 0.f : ml_s[k][row][1] * shaped_ex2(ml_s[k][row][0] - top);
+        mine[q][c] = top == -INFINITY ? 0.f : shaped_ex2(m[q][c] - top);
+        if (gi == 0 && g == 0) {
+          join[row * (D + 4) + D] = top;
+          join[row * (D + 4) + D + 1] = sum;
+        }
+      }
+    for (int k0 = 0; k0 < Cfg::GROUPS; k0 += Cfg::SLOTS) {
+      if (gi >= k0 && gi < k0 + Cfg::SLOTS) {
+#pragma unroll
+        for (int q = 0; q < NQ; ++q)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int row = (mt * NQ + q) * 8 + 2 * c4 + c;
+            if (row >= M) continue;
+            float* at = join + ((gi - k0) * Cfg::ROWS + row) * (D + 4) + g;
+            const float f = mine[q][c];
+#pragma unroll
+            for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                // a group none of whose keys is visible adds nothing, whatever its values are
+                const float v = f == 0.f ? 0.f : o[q][n][2 * h + c] * f;
+                at[n * 16 + 8 * h] = k0 == 0 ? v : at[n * 16 + 8 * h] + v;
+              }
+          }
       }
       named_bar(1, THREADS);
     }
-    const int w_first = step_owner(seq0, W, total), w_last = step_owner(seq1 - 1, W, total), R = M - m0;
+    if (Cfg::SLOTS > 1) {
+      for (int i = threadIdx.x; i < M * (D / 4); i += THREADS) {
+        float4* at = reinterpret_cast<float4*>(join + i / (D / 4) * (D + 4)) + i % (D / 4);
+        float4 v = *at;
+#pragma unroll
+        for (int k = 1; k < Cfg::SLOTS; ++k) {
+          const float4 u = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(at) + k * Cfg::ROWS * (D + 4));
+          v.x += u.x; v.y += u.y; v.z += u.z; v.w += u.w;
+        }
+        *at = v;
+      }
+      named_bar(1, THREADS);
+    }
+    const int w_first = step_owner(seq0, W, total), w_last = step_owner(seq1 - 1, W, total);
     bool finish = w_first == w_last;
     if (!finish) {
-      // part of worker v: row r of [rows_all], value n of [D + 2]
-      auto part = [&](int v) {
-        return p.parts + ((((size_t)v * 2 + (step_first(v, W, total) >= seq0 ? 0 : 1)) * p.Hkv + kvh) * rows_all + m0) * (D + 2);
-      };
-      float* to = part(w);
-      for (int i = threadIdx.x; i < R * (D + 2); i += THREADS) to[i] = join[i / (D + 2) * (D + 4) + i % (D + 2)];
+      // part of worker v: row r of [rows_all], values [D], maximum and sum
+      const bool ahead = step_first(w_first, W, total) < seq0;       // the first worker came from the sequence before
+      auto part = [&](int v) { return p.parts + ((size_t)(v * 2 + (v == w_first && ahead ? 1 : 0)) * p.Hkv + kvh) * M * (D + 4); };
+      float4* to = reinterpret_cast<float4*>(part(w));
+      for (int i = threadIdx.x; i < M * (D + 4) / 4; i += THREADS) to[i] = reinterpret_cast<const float4*>(join)[i];
       __threadfence();
       named_bar(1, THREADS);
       if (threadIdx.x == 0) {
@@ -454,42 +507,74 @@ __global__ void __launch_bounds__(StCfg<D, MT>::THREADS, 1) shaped_step_kernel(c
       }
       named_bar(1, THREADS);
       finish = S.last != 0;
-      if (finish) {                                                  // all parts are there
-        for (int r = warp; r < R; r += Cfg::WARPS) {                 // a warp per row
-          float big = -INFINITY;
-          for (int v = w_first + lane; v <= w_last; v += 32) big = fmaxf(big, __ldcg(part(v) + r * (D + 2) + D));
-          big = warp_max(big);
-          float acc[D / 32], den = 0.f;
+      if (finish) {                                                  // all parts are there; a warp per row, many loads in flight
+        for (int r = warp; r < M; r += Cfg::WARPS) {
+          constexpr int V = (148 + 31) / 32, B = 8, W4 = D / 128 > 0 ? D / 128 : 1;  // parts whose factors a lane holds, parts read at once
+          const int n = w_last - w_first + 1;
+          float f[V], den = 0.f, big = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < D / 32; ++n) acc[n] = 0.f;
-          for (int v = w_first; v <= w_last; ++v) {
-            const float* from = part(v) + r * (D + 2);
-            const float pm = __ldcg(from + D), f = pm == -INFINITY ? 0.f : shaped_ex2(pm - big);
-            den += f == 0.f ? 0.f : __ldcg(from + D + 1) * f;
-#pragma unroll
-            for (int n = 0; n < D / 32; ++n) acc[n] += f == 0.f ? 0.f : __ldcg(from + n * 32 + lane) * f;
+          for (int k = 0; k < V; ++k) {
+            const int v = k * 32 + lane;
+            f[k] = v < n ? __ldcg(part(w_first + v) + r * (D + 4) + D) : -INFINITY;
+            big = fmaxf(big, f[k]);
           }
-          float* at = join + r * (D + 4);
+          big = warp_max(big);
 #pragma unroll
-          for (int n = 0; n < D / 32; ++n) at[n * 32 + lane] = acc[n];
+          for (int k = 0; k < V; ++k) {
+            const int v = k * 32 + lane;
+            f[k] = f[k] == -INFINITY ? 0.f : shaped_ex2(f[k] - big);
+            if (f[k] != 0.f) den += __ldcg(part(w_first + v) + r * (D + 4) + D + 1) * f[k];
+          }
+          den = warp_sum(den);
+          float4 acc[W4];
+#pragma unroll
+          for (int k = 0; k < W4; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+          const bool mine = D >= 128 || lane < D / 4;
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            for (int v0 = k * 32; v0 < min(n, k * 32 + 32); v0 += B) {
+              float4 got[B][W4];
+#pragma unroll
+              for (int i = 0; i < B; ++i)
+#pragma unroll
+                for (int c = 0; c < W4; ++c)
+                  got[i][c] = mine ? __ldcg(reinterpret_cast<const float4*>(part(w_first + min(v0 + i, n - 1)) + r * (D + 4)) + c * 32 + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < B; ++i) {
+                const float fi = __shfl_sync(0xffffffffu, f[k], (v0 + i) & 31);        // zero behind the last part
+                if (fi != 0.f) {
+#pragma unroll
+                  for (int c = 0; c < W4; ++c) {
+                    acc[c].x = fmaf(got[i][c].x, fi, acc[c].x);
+                    acc[c].y = fmaf(got[i][c].y, fi, acc[c].y);
+                    acc[c].z = fmaf(got[i][c].z, fi, acc[c].z);
+                    acc[c].w = fmaf(got[i][c].w, fi, acc[c].w);
+                  }
+                }
+              }
+            }
+          float* at = join + r * (D + 4);
+          if (mine) {
+#pragma unroll
+            for (int c = 0; c < W4; ++c) reinterpret_cast<float4*>(at)[c * 32 + lane] = acc[c];
+          }
           if (lane == 0) { at[D] = big; at[D + 1] = den; }
         }
         named_bar(1, THREADS);
       }
     }
     if (finish) {
-      for (int i = threadIdx.x; i < R * (D / 2); i += THREADS) {
-        const int lr = i / (D / 2), r = m0 + lr, d = (i - lr * (D / 2)) * 2;
-        const float* at = join + lr * (D + 4);
+      for (int i = threadIdx.x; i < M * (D / 2); i += THREADS) {
+        const int r = i / (D / 2), d = (i - r * (D / 2)) * 2;
+        const float* at = join + r * (D + 4);
         const bool none = at[D] == -INFINITY && at[D + 1] == 0.f;
         const float inv = 1.f / at[D + 1];
         *reinterpret_cast<uint32_t*>(p.out + (size_t)(s * p.E + r / G) * p.ld_out + (size_t)(kvh * G + r % G) * D + d) =
             none ? 0u : st_pack(at[d] * inv, at[d + 1] * inv);
       }
       if (p.lse != nullptr || p.scores != nullptr)
-        for (int lr = threadIdx.x; lr < R; lr += THREADS) {
-          const float* at = join + lr * (D + 4);
-          const int r = m0 + lr;
+        for (int r = threadIdx.x; r < M; r += THREADS) {
+          const float* at = join + r * (D + 4);
           const bool none = at[D] == -INFINITY && at[D + 1] == 0.f;
           const float v = at[D] + __log2f(at[D + 1]);
           const size_t to = (size_t)(s * p.E + r / G) * p.Hq + kvh * G + r % G;
@@ -501,83 +586,91 @@ __global__ void __launch_bounds__(StCfg<D, MT>::THREADS, 1) shaped_step_kernel(c
   }
 }
 
-// mass[row, kvh, j] += sum over the rows of exp2(score - lse)
+// mass[row, kvh, j] += sum over the rows of exp2(score - lse); a warp takes one tile after the other
 __global__ void __launch_bounds__(256) shaped_step_mass_kernel(const ShapedStepParams p) {
   extern __shared__ int sm_tiles[];                                  // [bs + 1 + 32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, G = p.Hq / p.Hkv, M = p.E * G;
-  pdl_wait_prior_grid();
-  step_schedule(p, sm_tiles, sm_tiles + p.bs + 1);
+  step_schedule(p, sm_tiles, sm_tiles + p.bs + 1);                   // from what was there before the first kernel
   const int total = sm_tiles[p.bs];
   if (total > p.score_tiles) {                                       // the workspace is too small for these contexts
     if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
     return;
   }
-  for (int x = blockIdx.x * 8 + warp; x < total; x += gridDim.x * 8) {
-    const int s = step_sequence(sm_tiles, p.bs, x);
-    const StepKeys k = step_keys(p, s);
-    bool twice = false;                                              // a row listed twice would be added to by two warps at once
-    for (int o = lane; o < s; o += 32) twice |= p.rows[o] == k.row && p.lens[o] > 0;
-    if (__any_sync(0xffffffffu, twice)) {
-      if (lane == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
-      continue;
+  const int x = blockIdx.x * 8 + warp, many = gridDim.x * 8, pitch = (M + 3) / 4 * 4;
+  StepCursor cur;
+  cur.seq1 = -1;
+  bool twice = false;
+  pdl_wait_prior_grid();
+  for (int y = x; y < total; y += many) {
+    if (y >= cur.seq1) {
+      cur.seek(p, sm_tiles, y);
+      twice = false;                                                 // a row listed twice would be added to by two warps at once
+      for (int o = lane; o < cur.s; o += 32) twice |= p.rows[o] == cur.key.row && p.lens[o] > 0;
+      twice = __any_sync(0xffffffffu, twice);
+      if (twice && lane == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
     }
-    const int i = (x - sm_tiles[s]) * ST_K + 2 * lane;
-    const float* sc = p.scores + ((size_t)kvh * p.score_tiles + x) * M * ST_K + 2 * lane;
+    if (twice) continue;
+    const float* sc = p.scores + (((size_t)kvh * p.score_tiles + y) * ST_K + lane) * pitch;
+    const int i = (y - cur.seq0) * ST_K + lane;
+    float* to = p.mass + ((size_t)cur.key.row * p.Hkv + kvh) * p.mass_stride + cur.key.begin + i;
+    const float before0 = i < cur.key.n ? to[0] : 0.f, before1 = i + 32 < cur.key.n ? to[32] : 0.f;
     float a = 0.f, b = 0.f;
-    for (int r = 0; r < M; ++r) {
-      const float top = p.lse2[(size_t)(s * p.E + r / G) * p.Hq + kvh * G + r % G];
-      const float2 v = *reinterpret_cast<const float2*>(sc + (size_t)r * ST_K);
-      a += shaped_ex2(v.x - top);
-      b += shaped_ex2(v.y - top);
+    for (int r0 = 0; r0 < M; r0 += 4) {
+      const float4 u = *reinterpret_cast<const float4*>(sc + r0), v = *reinterpret_cast<const float4*>(sc + 32 * pitch + r0);
+      const float su[4] = {u.x, u.y, u.z, u.w}, sv[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int r = r0 + k;
+        const float top = r < M ? p.lse2[(size_t)(cur.s * p.E + r / G) * p.Hq + kvh * G + r % G] : INFINITY;
+        a += r < M ? shaped_ex2(su[k] - top) : 0.f;
+        b += r < M ? shaped_ex2(sv[k] - top) : 0.f;
+      }
     }
-    float* to = p.mass + ((size_t)k.row * p.Hkv + kvh) * p.mass_stride + k.begin + i;
-    if (i < k.n) to[0] += a;
-    if (i + 1 < k.n) to[1] += b;
+    if (i < cur.key.n) to[0] = before0 + a;
+    if (i + 32 < cur.key.n) to[32] = before1 + b;
   }
 }
 
 // Parts of the workspace, each from a 256-byte border.
 struct StepWork { size_t parts, lse2, scores, bytes; long long score_tiles, counted; int workers; };
 
-// Row tiles of a CTA: a warp's registers hold 16 rows of outputs; more than 32 rows go to further CTAs, which find the keys in L2.
-static int step_row_tiles(int M) { return M <= 16 ? 1 : 2; }
-
 static StepWork step_work(int bs, int E, int Hq, int Hkv, int D, long long keys) {
   StepWork w;
-  const int M = E * (Hq / Hkv), mt = step_row_tiles(M), blocks = (M + 16 * mt - 1) / (16 * mt);
-  w.workers = 148 / (Hkv * blocks) > 0 ? 148 / (Hkv * blocks) : 1;  // a CTA per SM
+  const int M = E * (Hq / Hkv);
+  w.workers = 148 / Hkv > 0 ? 148 / Hkv : 1;           // a CTA per SM
   w.score_tiles = keys > 0 ? keys / ST_K + bs : 0;                   // every sequence may end inside a tile
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  w.counted = (long long)bs * Hkv * blocks;
+  w.counted = (long long)bs * Hkv;
   w.parts = (size_t)ST_COUNTERS * 4;
-  w.lse2 = w.parts + up((size_t)w.workers * 2 * Hkv * M * (D + 2) * 4);
+  w.lse2 = w.parts + up((size_t)w.workers * 2 * Hkv * M * (D + 4) * 4);
   w.scores = w.lse2 + up((size_t)bs * E * Hq * 4);
-  w.bytes = w.scores + up((size_t)Hkv * w.score_tiles * M * ST_K * 4);
+  w.bytes = w.scores + up((size_t)Hkv * w.score_tiles * ((M + 3) / 4 * 4) * ST_K * 4);
   return w;
 }
 
-template <int D, int MT>
+template <int D, int NQ, int MT>
 static int launch_shaped_step(const ShapedStepParams& p, cudaStream_t st) {
-  using Cfg = StCfg<D, MT>;
-  static_assert(Cfg::SMEM + Cfg::GROUPS * 16 * MT * 8 + sizeof(StShared) <= 232448, "shared memory");
-  CUDA_CHECK_RET(cudaFuncSetAttribute(shaped_step_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::SMEM));
-  if constexpr (D == 256) {                           // what the warps ask for later is there from the start
-    static const int regs = [] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, shaped_step_kernel<D, MT>) == cudaSuccess ? a.numRegs : 0; }();
+  using Cfg = StCfg<D, NQ, MT>;
+  auto kernel = shaped_step_kernel<D, NQ, MT>;
+  static_assert(Cfg::SMEM + Cfg::GROUPS * Cfg::ROWS * 8 + Cfg::ROWS * 16 + sizeof(StShared) <= 232448, "shared memory");
+  CUDA_CHECK_RET(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::SMEM));
+  if constexpr (D == 256 && Cfg::THREADS == 384) {     // what the warps ask for later is there from the start
+    static const int regs = [&] { cudaFuncAttributes a; return cudaFuncGetAttributes(&a, kernel) == cudaSuccess ? a.numRegs : 0; }();
     if (regs < 168) return -155;
   }
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.workers, (unsigned)p.Hkv, (unsigned)((p.E * (p.Hq / p.Hkv) + 16 * MT - 1) / (16 * MT)));
+  cfg.gridDim = dim3((unsigned)p.workers, (unsigned)p.Hkv);
   cfg.blockDim = dim3(Cfg::THREADS);
   cfg.dynamicSmemBytes = Cfg::SMEM;
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = p.pdl ? 1 : 0;
-  CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, shaped_step_kernel<D, MT>, p));
+  CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, kernel, p));
   if (p.mass == nullptr) return 0;
-  cfg.gridDim = dim3((unsigned)((296 + p.Hkv - 1) / p.Hkv), (unsigned)p.Hkv);
+  cfg.gridDim = dim3((unsigned)((148 * 4 + p.Hkv - 1) / p.Hkv), (unsigned)p.Hkv);
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = (size_t)(p.bs + 1 + 32) * 4;
   cfg.numAttrs = 1;
@@ -611,7 +704,7 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
   if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -152;
   if (mass != nullptr && mass_stride < bt_stride) return -153;
   StepWork w = step_work(bs, E, Hq, Hkv, D, 0);
-  if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hq * E * ST_K * 4);       // the rest of it
+  if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hkv * ((E * (Hq / Hkv) + 3) / 4 * 4) * ST_K * 4);       // the rest of it
   if (work_bytes < (long long)w.bytes || (mass != nullptr && w.score_tiles < 1)) return -154;
   ShapedStepParams p;
   p.c = ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, scale, cap};
@@ -622,11 +715,13 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
   p.scores = mass != nullptr ? (float*)(base + w.scores) : nullptr;
   p.ld_q = ld_q; p.ld_out = ld_out; p.mass_stride = mass_stride; p.score_tiles = w.score_tiles;
   p.bs = bs; p.E = E; p.Hq = Hq; p.Hkv = Hkv; p.workers = w.workers; p.pdl = pdl; p.status = status;
-  const int mt = step_row_tiles(E * (Hq / Hkv));
-#define SMC_SHAPED_STEP(DD)                                      \
-  if (D == DD) {                                                 \
-    if (mt == 1) return launch_shaped_step<DD, 1>(p, st);        \
-    return launch_shaped_step<DD, 2>(p, st);                     \
+  const int rows_each = E * (Hq / Hkv);
+#define SMC_SHAPED_STEP(DD)                                                  \
+  if (D == DD) {                                                             \
+    if (rows_each <= 8) return launch_shaped_step<DD, 1, 1>(p, st);          \
+    if (rows_each <= 16) return launch_shaped_step<DD, 2, 1>(p, st);         \
+    if (rows_each <= 32) return launch_shaped_step<DD, 2, 2>(p, st);         \
+    return launch_shaped_step<DD, 2, 4>(p, st);                              \
   }
   SMC_SHAPED_STEP(64)
   SMC_SHAPED_STEP(128)
