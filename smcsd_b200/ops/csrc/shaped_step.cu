@@ -1,7 +1,7 @@
 // Attention of single tokens, or a few of each sequence, over the paged cache with capped, distance-biased or interval-masked scores
 // (shaped.cuh), and the weight that every cached token collects in it.
 //
-// What bounds it is the cache: 4 D bytes per key and KV head, read once.  The keys of all sequences, cut into tiles of 64, are one line of
+// What bounds it is the cache: 4 D bytes per key and KV head, read once.  The keys of all sequences, cut into tiles of 64 (128 with D = 64), are one line of
 // work per KV head that W workers share in equal parts, wherever sequences begin and end: a batch of ragged contexts keeps every SM busy to the
 // end, and a single sequence is spread over all of them.  Four loader warps gather the tiles page by page with cp.async into a ring; the other
 // warps take 16 keys each, two tiles in turn, and come to the loaders' ring only through its barriers.
@@ -22,7 +22,9 @@ namespace smc {
 // Registers of 384 threads, 168 each at the start: the loaders leave theirs to the warps that hold outputs.
 constexpr int ST_FEW = 40, ST_MANY = 232;
 static_assert(128 * ST_FEW + 256 * ST_MANY <= 384 * 168, "the registers of the launch");
-constexpr int ST_K = 64, ST_MAX_BS = 1024, ST_LOADERS = 4;
+constexpr int ST_MAX_BS = 1024, ST_LOADERS = 4;
+// Keys of a tile: what a loader warp does besides copying comes once a tile, and 64 keys of 128 bytes were too few to hide it (108 us against 4373 GB/s).
+constexpr int step_tile(int D) { return D == 64 ? 128 : 64; }
 constexpr int ST_COUNTERS = 32768;                     // at the front of every workspace, whatever batch it serves next
 
 struct ShapedStepParams {
@@ -39,9 +41,9 @@ struct ShapedStepParams {
   int* counters;                 // [row blocks][bs][Hkv], zero between calls
   float* parts;                  // [W][2][Hkv][E G][D + 4]
   float* lse2;                   // [bs * E, Hq] in base 2, +inf where nothing is visible
-  float* scores;                 // [Hkv][score_tiles][64][pitch], pitch E G rounded up to 4
+  float* scores;                 // [Hkv][score_tiles][tile][pitch], pitch E G rounded up to 4
   long long ld_q, ld_out, mass_stride, score_tiles;
-  int bs, E, Hq, Hkv, workers, pdl;
+  int bs, E, Hq, Hkv, workers, tile, pdl;
   int* status;
 };
 
@@ -86,9 +88,6 @@ __device__ __forceinline__ int step_owner(int x, int workers, int total) { retur
 __device__ __forceinline__ void st_cp16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void st_cp4(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void st_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -116,7 +115,7 @@ __device__ __forceinline__ void step_schedule(const ShapedStepParams& p, int* ti
   int base = 0;
   for (int s0 = 0; s0 < p.bs; s0 += blockDim.x) {
     const int s = s0 + threadIdx.x;
-    int sum = s < p.bs ? (step_keys(p, s).n + ST_K - 1) / ST_K : 0;
+    int sum = s < p.bs ? (step_keys(p, s).n + p.tile - 1) / p.tile : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -152,14 +151,16 @@ template <int D, int NQ, int MT>
 struct StCfg {
   static constexpr int ROWS = 8 * NQ * MT;
   // groups of keys in a tile, tiles in turn: eight consumer warps; four with D = 256, whose 16 keys a warp holds while it works are 16 KB
-  static constexpr int GW = MT == 4 ? 2 : 4, SUB = 4 / GW, TURNS = MT == 1 && D < 256 ? 2 : 1;
+  static constexpr int KT = step_tile(D), TURNS = MT == 1 && D == 128 ? 2 : 1, GW = MT == 1 ? (D == 64 ? 8 : 4) : MT == 2 ? 4 : 2, SUB = KT / 16 / GW;
   static constexpr int GROUPS = GW * TURNS, WARPS = GROUPS * MT, THREADS = (WARPS + ST_LOADERS) * 32;
   static constexpr int LD = D + 8;
-  static constexpr int STAGES = D == 64 ? 8 : D == 128 ? 5 : MT == 1 ? 3 : 2;
+  static constexpr int STAGES = D == 64 ? 4 : D == 128 ? 5 : MT == 1 ? 3 : 2;
+  // rows of 512 bytes come as one bulk copy each (19 cycles a copy, whatever its size); shorter ones in pieces of 16 bytes
+  static constexpr bool BULK = D == 256;
   static constexpr int SLOTS = D == 256 ? (ROWS == 8 ? 2 : 1) : 64 / ROWS;           // states that groups leave at once when they are joined
-  static constexpr size_t KV = (size_t)ST_K * LD * 2;                // one of K, V
+  static constexpr size_t KV = (size_t)KT * LD * 2;                // one of K, V
   // stages, states, positions of the tiles in flight, prefix sums
-  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)SLOTS * ROWS * (D + 4) * 4 + (size_t)STAGES * ST_K * 4 + (ST_MAX_BS + 1 + 64) * 4;
+  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)SLOTS * ROWS * (D + 4) * 4 + (size_t)STAGES * KT * 4 + (ST_MAX_BS + 1 + 64) * 4;
 };
 
 // A place in the line of tiles: the sequence that tile x belongs to.
@@ -198,12 +199,13 @@ __device__ __forceinline__ bool st_wait(StShared& S, int* status, uint64_t* bar,
 template <int D, int NQ, int MT>
 __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kernel(const ShapedStepParams p) {
   using Cfg = StCfg<D, NQ, MT>;
-  constexpr int LD = Cfg::LD, STAGES = Cfg::STAGES, THREADS = Cfg::WARPS * 32, CPR = D / 8;
+  constexpr int LD = Cfg::LD, KT = Cfg::KT, KW = KT / ST_LOADERS, STAGES = Cfg::STAGES, THREADS = Cfg::WARPS * 32;
+  [[maybe_unused]] constexpr int CPR = D / 8;
   extern __shared__ __align__(128) uint8_t st_smem[];
-  __nv_bfloat16* kv_s = reinterpret_cast<__nv_bfloat16*>(st_smem);   // [stage][K, V][64][LD]
+  __nv_bfloat16* kv_s = reinterpret_cast<__nv_bfloat16*>(st_smem);   // [stage][K, V][KT][LD]
   float* join = reinterpret_cast<float*>(st_smem + STAGES * 2 * Cfg::KV);            // [slot][ROWS][D + 4]
-  int* pos_s = reinterpret_cast<int*>(join + Cfg::SLOTS * Cfg::ROWS * (D + 4));      // [stage][64]
-  int* tiles = pos_s + STAGES * ST_K;                                // [bs + 1]
+  int* pos_s = reinterpret_cast<int*>(join + Cfg::SLOTS * Cfg::ROWS * (D + 4));      // [stage][KT]
+  int* tiles = pos_s + STAGES * KT;                                  // [bs + 1]
   int* misc = tiles + ST_MAX_BS + 1;                                 // [64]
   __shared__ float ml_s[Cfg::GROUPS][Cfg::ROWS][2];
   __shared__ float4 row_s[Cfg::ROWS];                                // of a row: first and last visible position, its own, slope
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
   int* counter = p.counters + kvh;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&S.full[i], ST_LOADERS * 32);
+      mbar_init(&S.full[i], Cfg::BULK ? ST_LOADERS : ST_LOADERS * 32);
       mbar_init(&S.empty[i], Cfg::GW * MT);
     }
     S.abort = 0;
@@ -246,47 +248,81 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
 
   if (warp >= Cfg::WARPS) {
     if constexpr (D == 256 && Cfg::THREADS == 384) regs_fewer<ST_FEW>();
-    // ================================================================= loaders: 16 keys of each tile a warp
-    const int lw = warp - Cfg::WARPS, kl0 = lw * 16 + (lane & 15);
-    const size_t kv_row = (size_t)p.Hkv * D;
-    constexpr int AHEAD = 3;                                         // tiles that page ids are read ahead
-    StepCursor cur;
-    cur.seq1 = t_begin;
-    int page[AHEAD], from[AHEAD];                                    // of this lane's key: page, index of its position or -1
-    auto ids = [&](int x, int& pg, int& at) {
-      if (x >= t_end) return;
-      if (x >= cur.seq1) cur.seek(p, tiles, x);
-      const int i = (x - cur.seq0) * ST_K + kl0, idx = cur.key.begin + min(i, cur.key.n - 1);       // keys behind the last repeat it
-      pg = p.c.block_table[(size_t)cur.key.row * p.c.bt_stride + idx];
-      at = cur.key.row * p.c.kp_stride + idx;
+    // ================================================================= loaders: KW keys of each tile a warp
+    const int lw = warp - Cfg::WARPS, kl0 = lw * KW + lane % KW;
+    const long long row_bytes = (long long)p.Hkv * D * 2;
+    // what this lane copies: with BULK a row of K or V, else chunk lane % CPR of the rows lane / CPR, + 32 / CPR, ...
+    const int c = Cfg::BULK ? 0 : lane % CPR, r0 = Cfg::BULK ? lane & 15 : lane / CPR;
+    const char* from_k = reinterpret_cast<const char*>((Cfg::BULK && lane >= 16 ? p.v_pool : p.k_pool) + (size_t)kvh * D + c * 8);
+    const char* from_v = reinterpret_cast<const char*>(p.v_pool + (size_t)kvh * D + c * 8);
+    const uint32_t to0 = smem_u32(kv_s) + (uint32_t)((lw * KW + r0) * LD + c * 8) * 2 + (Cfg::BULK && lane >= 16 ? (uint32_t)Cfg::KV : 0u);
+    constexpr int AHEAD = 4;                                         // tiles that page ids are read ahead
+    int page[AHEAD], kpos[AHEAD];                                    // of this lane's key
+    int next = t_begin, seq_end = t_begin, i = 0, n = 0;             // next tile to read ids of; this lane's key among the n of its sequence
+    const int* bt = nullptr;
+    const int* kp = nullptr;
+    auto ids = [&](int& pg, int& pos) {
+      if (next >= t_end) return;
+      if (next >= seq_end) {
+        StepCursor cur;
+        cur.seek(p, tiles, next);
+        seq_end = cur.seq1;
+        n = cur.key.n;
+        i = (next - cur.seq0) * KT + kl0;
+        bt = p.c.block_table + (size_t)cur.key.row * p.c.bt_stride + cur.key.begin;
+        if (p.c.key_pos != nullptr) kp = p.c.key_pos + (size_t)cur.key.row * p.c.kp_stride + cur.key.begin;
+      }
+      const int at = min(i, n - 1);                                  // keys behind the last repeat it
+      pg = bt[at];
+      if (kp != nullptr) pos = kp[at];
+      i += KT;
+      ++next;
     };
 #pragma unroll
-    for (int d = 0; d < AHEAD; ++d) ids(t_begin + d, page[d], from[d]);
-    for (int x0 = t_begin; x0 < t_end; x0 += AHEAD) {
+    for (int d = 0; d < AHEAD; ++d) ids(page[d], kpos[d]);
+    int st = 0, left = t_end - t_begin;
+    uint32_t phase = 1;                                              // of the stage's last release; the first use waits for none
+    bool ok = true;
+    while (left > 0 && ok) {
 #pragma unroll
       for (int d = 0; d < AHEAD; ++d) {
-        const int x = x0 + d, n = x - t_begin, st = n % STAGES;
-        if (x >= t_end) break;
+        if (left <= 0) break;
         int pg = page[d];
-        const int at = from[d];
-        if (pg < 0 || pg > p.c.n_pages) { atomicOr(p.status, SMC_ERR_BOUNDS); pg = 0; }
-        ids(x + AHEAD, page[d], from[d]);
-        const bool ok = n < STAGES || st_wait(S, p.status, &S.empty[st], (uint32_t)(n / STAGES - 1) & 1u);
-        if (!__all_sync(0xffffffffu, ok)) { x0 = t_end; break; }
-        const uint32_t k0 = smem_u32(kv_s + (size_t)st * 2 * ST_K * LD);
-#pragma unroll 8
-        for (int i = lane; i < 16 * CPR; i += 32) {
-          const int kl = i / CPR, c = i - kl * CPR;
-          const size_t src = (size_t)__shfl_sync(0xffffffffu, pg, kl) * kv_row + (size_t)kvh * D + c * 8;
-          const uint32_t dst = k0 + (uint32_t)((lw * 16 + kl) * LD + c * 8) * 2;
-          st_cp16(dst, p.k_pool + src);
-          st_cp16(dst + (uint32_t)Cfg::KV, p.v_pool + src);
+        const int pos = kpos[d];
+        if ((unsigned)pg > (unsigned)p.c.n_pages) { atomicOr(p.status, SMC_ERR_BOUNDS); pg = 0; }
+        ids(page[d], kpos[d]);
+        ok = __all_sync(0xffffffffu, st_wait(S, p.status, &S.empty[st], phase));
+        if (!ok) break;
+        if (kp != nullptr && lane < KW) pos_s[st * KT + kl0] = pos;
+        const uint32_t to = to0 + (uint32_t)st * (uint32_t)(2 * Cfg::KV);
+        if constexpr (Cfg::BULK) {
+          __syncwarp();
+          if (lane == 0) mbar_expect_tx(&S.full[st], 32 * D * 2);
+          __syncwarp();
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                       ::"r"(to), "l"(from_k + pg * row_bytes), "r"(D * 2), "r"(smem_u32(&S.full[st])) : "memory");
+        } else {
+#pragma unroll
+          for (int r = 0; r < KW; r += 32 / CPR) {
+            const long long off = __shfl_sync(0xffffffffu, pg, r0 + r) * row_bytes;
+            st_cp16(to + (uint32_t)(r * LD * 2), from_k + off);
+            st_cp16(to + (uint32_t)(r * LD * 2) + (uint32_t)Cfg::KV, from_v + off);
+          }
+          __syncwarp();                                              // each lane arrives once its own copies have landed
+          asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&S.full[st])) : "memory");
         }
-        if (p.c.key_pos != nullptr && lane < 16) st_cp4(smem_u32(pos_s + st * ST_K + kl0), p.c.key_pos + at);
-        asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&S.full[st])) : "memory");       // when all of them have landed
+        --left;
+        if (++st == STAGES) { st = 0; phase ^= 1u; }
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
+    if constexpr (Cfg::BULK) {
+      // a CTA that gave up keeps its shared memory until the copies in flight have landed
+      const int issued = t_end - t_begin - left;
+      if (S.abort)
+        for (int k = max(0, issued - STAGES); k < issued; ++k) (void)mbar_wait(&S.full[k % STAGES], (uint32_t)(k / STAGES) & 1u);
+    } else {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+    }
     return;
   }
 
@@ -339,8 +375,8 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
 #pragma unroll
       for (int sub = 0; sub < Cfg::SUB; ++sub) {
         const int k0 = (kg * Cfg::SUB + sub) * 16;
-        const __nv_bfloat16* Kt = kv_s + (size_t)st * 2 * ST_K * LD + k0 * LD;
-        const __nv_bfloat16* Vt = Kt + ST_K * LD;
+        const __nv_bfloat16* Kt = kv_s + (size_t)st * 2 * KT * LD + k0 * LD;
+        const __nv_bfloat16* Vt = Kt + KT * LD;
         float sc[NQ][4], sd[NQ][4];                                  // two chains of products
 #pragma unroll
         for (int q = 0; q < NQ; ++q) sc[q][0] = sc[q][1] = sc[q][2] = sc[q][3] = sd[q][0] = sd[q][1] = sd[q][2] = sd[q][3] = 0.f;
@@ -357,11 +393,11 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
             st_mma(sd[q], b, qb[q][kk + 1][0], qb[q][kk + 1][1]);
           }
         }
-        const int i0 = (x - seq0) * ST_K + k0 + g;                   // of the sequence's visible keys: this lane's, and the one 8 behind
+        const int i0 = (x - seq0) * KT + k0 + g;                     // of the sequence's visible keys: this lane's, and the one 8 behind
         float kp[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int pos = p.c.key_pos != nullptr ? pos_s[st * ST_K + k0 + g + 8 * h] : key.begin + i0 + 8 * h;
+          const int pos = p.c.key_pos != nullptr ? pos_s[st * KT + k0 + g + 8 * h] : key.begin + i0 + 8 * h;
           kp[h] = i0 + 8 * h < key.n ? (float)pos : -1.f;
         }
         uint32_t pb[NQ][2];
@@ -380,7 +416,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
           }
           if (p.scores != nullptr && x < p.score_tiles) {
             const int r = (mt * NQ + q) * 8 + 2 * c4;
-            float* at = p.scores + (((size_t)kvh * p.score_tiles + x) * ST_K + k0 + g) * pitch + r;
+            float* at = p.scores + (((size_t)kvh * p.score_tiles + x) * KT + k0 + g) * pitch + r;
             if (r < pitch) {
               *reinterpret_cast<float2*>(at) = make_float2(sc[q][0], sc[q][1]);
               *reinterpret_cast<float2*>(at + 8 * pitch) = make_float2(sc[q][2], sc[q][3]);
@@ -610,24 +646,26 @@ __global__ void __launch_bounds__(256) shaped_step_mass_kernel(const ShapedStepP
       if (twice && lane == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
     }
     if (twice) continue;
-    const float* sc = p.scores + (((size_t)kvh * p.score_tiles + y) * ST_K + lane) * pitch;
-    const int i = (y - cur.seq0) * ST_K + lane;
-    float* to = p.mass + ((size_t)cur.key.row * p.Hkv + kvh) * p.mass_stride + cur.key.begin + i;
-    const float before0 = i < cur.key.n ? to[0] : 0.f, before1 = i + 32 < cur.key.n ? to[32] : 0.f;
-    float a = 0.f, b = 0.f;
-    for (int r0 = 0; r0 < M; r0 += 4) {
-      const float4 u = *reinterpret_cast<const float4*>(sc + r0), v = *reinterpret_cast<const float4*>(sc + 32 * pitch + r0);
-      const float su[4] = {u.x, u.y, u.z, u.w}, sv[4] = {v.x, v.y, v.z, v.w};
+    for (int k0 = lane; k0 < p.tile; k0 += 64) {
+      const float* sc = p.scores + (((size_t)kvh * p.score_tiles + y) * p.tile + k0) * pitch;
+      const int i = (y - cur.seq0) * p.tile + k0;
+      float* to = p.mass + ((size_t)cur.key.row * p.Hkv + kvh) * p.mass_stride + cur.key.begin + i;
+      const float before0 = i < cur.key.n ? to[0] : 0.f, before1 = i + 32 < cur.key.n ? to[32] : 0.f;
+      float a = 0.f, b = 0.f;
+      for (int r0 = 0; r0 < M; r0 += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(sc + r0), v = *reinterpret_cast<const float4*>(sc + 32 * pitch + r0);
+        const float su[4] = {u.x, u.y, u.z, u.w}, sv[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int r = r0 + k;
-        const float top = r < M ? p.lse2[(size_t)(cur.s * p.E + r / G) * p.Hq + kvh * G + r % G] : INFINITY;
-        a += r < M ? shaped_ex2(su[k] - top) : 0.f;
-        b += r < M ? shaped_ex2(sv[k] - top) : 0.f;
+        for (int k = 0; k < 4; ++k) {
+          const int r = r0 + k;
+          const float top = r < M ? p.lse2[(size_t)(cur.s * p.E + r / G) * p.Hq + kvh * G + r % G] : INFINITY;
+          a += r < M ? shaped_ex2(su[k] - top) : 0.f;
+          b += r < M ? shaped_ex2(sv[k] - top) : 0.f;
+        }
       }
+      if (i < cur.key.n) to[0] = before0 + a;
+      if (i + 32 < cur.key.n) to[32] = before1 + b;
     }
-    if (i < cur.key.n) to[0] = before0 + a;
-    if (i + 32 < cur.key.n) to[32] = before1 + b;
   }
 }
 
@@ -638,13 +676,13 @@ static StepWork step_work(int bs, int E, int Hq, int Hkv, int D, long long keys)
   StepWork w;
   const int M = E * (Hq / Hkv);
   w.workers = 148 / Hkv > 0 ? 148 / Hkv : 1;           // a CTA per SM
-  w.score_tiles = keys > 0 ? keys / ST_K + bs : 0;                   // every sequence may end inside a tile
+  w.score_tiles = keys > 0 ? keys / step_tile(D) + bs : 0;                   // every sequence may end inside a tile
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   w.counted = (long long)bs * Hkv;
   w.parts = (size_t)ST_COUNTERS * 4;
   w.lse2 = w.parts + up((size_t)w.workers * 2 * Hkv * M * (D + 4) * 4);
   w.scores = w.lse2 + up((size_t)bs * E * Hq * 4);
-  w.bytes = w.scores + up((size_t)Hkv * w.score_tiles * ((M + 3) / 4 * 4) * ST_K * 4);
+  w.bytes = w.scores + up((size_t)Hkv * w.score_tiles * ((M + 3) / 4 * 4) * step_tile(D) * 4);
   return w;
 }
 
@@ -704,7 +742,7 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
   if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -152;
   if (mass != nullptr && mass_stride < bt_stride) return -153;
   StepWork w = step_work(bs, E, Hq, Hkv, D, 0);
-  if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hkv * ((E * (Hq / Hkv) + 3) / 4 * 4) * ST_K * 4);       // the rest of it
+  if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hkv * ((E * (Hq / Hkv) + 3) / 4 * 4) * step_tile(D) * 4);       // the rest of it
   if (work_bytes < (long long)w.bytes || (mass != nullptr && w.score_tiles < 1)) return -154;
   ShapedStepParams p;
   p.c = ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, scale, cap};
@@ -714,7 +752,7 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
   p.counters = (int*)base; p.parts = (float*)(base + w.parts); p.lse2 = (float*)(base + w.lse2);
   p.scores = mass != nullptr ? (float*)(base + w.scores) : nullptr;
   p.ld_q = ld_q; p.ld_out = ld_out; p.mass_stride = mass_stride; p.score_tiles = w.score_tiles;
-  p.bs = bs; p.E = E; p.Hq = Hq; p.Hkv = Hkv; p.workers = w.workers; p.pdl = pdl; p.status = status;
+  p.bs = bs; p.E = E; p.Hq = Hq; p.Hkv = Hkv; p.workers = w.workers; p.tile = step_tile(D); p.pdl = pdl; p.status = status;
   const int rows_each = E * (Hq / Hkv);
 #define SMC_SHAPED_STEP(DD)                                                  \
   if (D == DD) {                                                             \
