@@ -622,50 +622,63 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
   }
 }
 
-// mass[row, kvh, j] += sum over the rows of exp2(score - lse); a warp takes one tile after the other
-__global__ void __launch_bounds__(256) shaped_step_mass_kernel(const ShapedStepParams p) {
+// mass[row, kvh, j] += sum over the rows of exp2(score - lse).  Every warp takes an equal run of tiles, a lane a key; four keys of a lane are in
+// flight at once (one tile after the other, each looked up anew, took 27 us for the 230,000 keys and 8 heads that take %s now).
+constexpr int SM_WARPS = 8;
+
+__global__ void __launch_bounds__(SM_WARPS * 32) shaped_step_mass_kernel(const ShapedStepParams p) {
   extern __shared__ int sm_tiles[];                                  // [bs + 1 + 32]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, G = p.Hq / p.Hkv, M = p.E * G;
+  __shared__ __align__(16) float top_s[SM_WARPS][64];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, G = p.Hq / p.Hkv, M = p.E * G, pitch = (M + 3) / 4 * 4;
   step_schedule(p, sm_tiles, sm_tiles + p.bs + 1);                   // from what was there before the first kernel
-  const int total = sm_tiles[p.bs];
+  const int total = sm_tiles[p.bs], many = gridDim.x * SM_WARPS, me = blockIdx.x * SM_WARPS + warp;
   if (total > p.score_tiles) {                                       // the workspace is too small for these contexts
     if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
     return;
   }
-  const int x = blockIdx.x * 8 + warp, many = gridDim.x * 8, pitch = (M + 3) / 4 * 4;
-  StepCursor cur;
-  cur.seq1 = -1;
-  bool twice = false;
+  const int x_end = step_first(me + 1, many, total);
+  int x = step_first(me, many, total);
   pdl_wait_prior_grid();
-  for (int y = x; y < total; y += many) {
-    if (y >= cur.seq1) {
-      cur.seek(p, sm_tiles, y);
-      twice = false;                                                 // a row listed twice would be added to by two warps at once
-      for (int o = lane; o < cur.s; o += 32) twice |= p.rows[o] == cur.key.row && p.lens[o] > 0;
-      twice = __any_sync(0xffffffffu, twice);
-      if (twice && lane == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
+  while (x < x_end) {
+    StepCursor cur;
+    cur.seek(p, sm_tiles, x);
+    const int end = min(x_end, cur.seq1);
+    bool twice = false;                                              // a row listed twice would be added to by two warps at once
+    for (int o = lane; o < cur.s; o += 32) twice |= p.rows[o] == cur.key.row && p.lens[o] > 0;
+    if (__any_sync(0xffffffffu, twice)) {
+      if (lane == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
+      x = end;
+      continue;
     }
-    if (twice) continue;
-    for (int k0 = lane; k0 < p.tile; k0 += 64) {
-      const float* sc = p.scores + (((size_t)kvh * p.score_tiles + y) * p.tile + k0) * pitch;
-      const int i = (y - cur.seq0) * p.tile + k0;
-      float* to = p.mass + ((size_t)cur.key.row * p.Hkv + kvh) * p.mass_stride + cur.key.begin + i;
-      const float before0 = i < cur.key.n ? to[0] : 0.f, before1 = i + 32 < cur.key.n ? to[32] : 0.f;
-      float a = 0.f, b = 0.f;
-      for (int r0 = 0; r0 < M; r0 += 4) {
-        const float4 u = *reinterpret_cast<const float4*>(sc + r0), v = *reinterpret_cast<const float4*>(sc + 32 * pitch + r0);
-        const float su[4] = {u.x, u.y, u.z, u.w}, sv[4] = {v.x, v.y, v.z, v.w};
+    __syncwarp();
+    for (int r = lane; r < pitch; r += 32)
+      top_s[warp][r] = r < M ? p.lse2[(size_t)(cur.s * p.E + r / G) * p.Hq + kvh * G + r % G] : INFINITY;
+    __syncwarp();
+    const float* sc = p.scores + ((size_t)kvh * p.score_tiles + cur.seq0) * p.tile * pitch;
+    float* to = p.mass + ((size_t)cur.key.row * p.Hkv + kvh) * p.mass_stride + cur.key.begin;
+    const int i_end = min((end - cur.seq0) * p.tile, cur.key.n);
+    for (int i = (x - cur.seq0) * p.tile + lane; i < i_end; i += 128) {
+      float sum[4] = {0.f, 0.f, 0.f, 0.f}, before[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int r = r0 + k;
-          const float top = r < M ? p.lse2[(size_t)(cur.s * p.E + r / G) * p.Hq + kvh * G + r % G] : INFINITY;
-          a += r < M ? shaped_ex2(su[k] - top) : 0.f;
-          b += r < M ? shaped_ex2(sv[k] - top) : 0.f;
+      for (int k = 0; k < 4; ++k) before[k] = i + 32 * k < i_end ? to[i + 32 * k] : 0.f;
+      for (int r = 0; r < pitch; r += 4) {
+        const float4 top = *reinterpret_cast<const float4*>(&top_s[warp][r]);
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const float4*>(sc + (size_t)min(i + 32 * k, i_end - 1) * pitch + r);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {                                // columns behind the last row were never written
+          sum[k] += shaped_ex2(v[k].x - top.x);
+          sum[k] += r + 1 < M ? shaped_ex2(v[k].y - top.y) : 0.f;
+          sum[k] += r + 2 < M ? shaped_ex2(v[k].z - top.z) : 0.f;
+          sum[k] += r + 3 < M ? shaped_ex2(v[k].w - top.w) : 0.f;
         }
       }
-      if (i < cur.key.n) to[0] = before0 + a;
-      if (i + 32 < cur.key.n) to[32] = before1 + b;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + 32 * k < i_end) to[i + 32 * k] = before[k] + sum[k];
     }
+    x = end;
   }
 }
 
@@ -709,7 +722,7 @@ static int launch_shaped_step(const ShapedStepParams& p, cudaStream_t st) {
   CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, kernel, p));
   if (p.mass == nullptr) return 0;
   cfg.gridDim = dim3((unsigned)((148 * 4 + p.Hkv - 1) / p.Hkv), (unsigned)p.Hkv);
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(SM_WARPS * 32);
   cfg.dynamicSmemBytes = (size_t)(p.bs + 1 + 32) * 4;
   cfg.numAttrs = 1;
   CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, shaped_step_mass_kernel, p));
