@@ -40,7 +40,7 @@ struct ShapedPromptParams {
 
 template <int D> struct SpShared {
   static constexpr int SLOTS = SpCfg<D>::UNITS / 2 + 1;               // steps whose keys' positions are held
-  uint64_t kv_full[SpCfg<D>::UNITS], kv_empty[SpCfg<D>::UNITS], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], pos_full[SLOTS];
+  uint64_t kv_full[SpCfg<D>::UNITS], kv_empty[SpCfg<D>::UNITS], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], pos_full[SLOTS], turn[2][4];
   alignas(16) float pos[SLOTS][SpCfg<D>::BK];
   uint32_t tmem_slot;
   int lo[8], hi[8], begin, end[2];
@@ -167,6 +167,7 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
     for (int s = 0; s < SLOTS; ++s) mbar_init(&S.pos_full[s], SP_LOADERS);
     for (int t = 0; t < NT; ++t) {
       mbar_init(&S.q_full[t], 4);
+      for (int q = 0; q < 4; ++q) mbar_init(&S.turn[t][q], 1);
       for (int i = 0; i < SB; ++i) {
         mbar_init(&S.s_full[t][i], 1);
         mbar_init(&S.p_full[t][i], 4);
@@ -475,6 +476,14 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
       }
       if (grow) m_ref = top;
       const float ref = m_ref == -INFINITY ? 0.f : m_ref;             // a row that has seen nothing yet: every probability is exp2(-inf)
+      // The two warps that share a scheduler (same quarter of either tile) take turns at the exponentials, tile 0 first: one waits for its scores and
+      // looks for its maxima meanwhile.
+      if (NT > 1) {
+        const int q = warp & 3;
+        const bool in_turn = t ? j >= n_of[0] || sp_wait(S, p.status, &S.turn[1][q], (uint32_t)j & 1u)
+                               : j == 0 || j > n_of[1] || sp_wait(S, p.status, &S.turn[0][q], (uint32_t)(j - 1) & 1u);
+        if (!__all_sync(0xffffffffu, in_turn)) { alive = false; break; }
+      }
       const uint64_t mul2 = f2_pair(mul, mul), off = f2_pair(-ref, -ref);
 #pragma unroll
       for (int c0 = 0; c0 < BK; c0 += 32) {
@@ -488,6 +497,7 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
         }
         tmem_st_32x32b_x16(ts + (c0 >> 1), pk);
       }
+      if (NT > 1 && lane == 0) mbar_arrive(&S.turn[t ^ 1][warp & 3]);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
