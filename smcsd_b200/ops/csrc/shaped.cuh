@@ -21,8 +21,17 @@ struct ShapedCache {
   const int2* bounds;            // per query token: first and last visible position, or null: all up to its own
   const float* slopes;           // per query head, or null
   int bt_stride, bt_rows, kp_stride, n_pages;
-  float scale, cap;
+  float mul;                     // scale log2(e)
+  float cap_in, cap_out;         // scale / cap and cap log2(e), 0: no cap
 };
+
+// (in double precision: an error of a factor is one of every score)
+inline ShapedCache shaped_cache(const int* block_table, int bt_stride, int bt_rows, int n_pages, const int* key_pos, int kp_stride, const int* bounds,
+                                const float* slopes, float scale, float cap) {
+  const double log2e = 1.4426950408889634;
+  return ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, (float)(scale * log2e),
+                     cap > 0.f ? (float)((double)scale / cap) : 0.f, cap > 0.f ? (float)(cap * log2e) : 0.f};
+}
 
 // One sequence of a call: block-table row, tokens held before the new ones, index of the first new one in q, new tokens.
 struct ShapedRun { int row, held, at, n; };
@@ -75,6 +84,14 @@ __device__ __forceinline__ float shaped_ex2(float x) {
 template <int N> __device__ __forceinline__ void regs_fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// one column of tensor memory, a number per lane
+__device__ __forceinline__ void tmem_ld_32x32b_x1(uint32_t taddr, uint32_t& r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_32x32b_x1(uint32_t taddr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r));
+}
+
 // two fp32 operations at once
 __device__ __forceinline__ uint64_t f2_pair(float a, float b) {
   uint64_t y;
@@ -107,25 +124,33 @@ __device__ __forceinline__ float shaped_max3(float a, float b, float c) {
   return y;
 }
 
-// tanh u = u P(u^2) for u^2 <= SH_TANH_MAX: minimax polynomials of tanh(sqrt y) / sqrt y on [0, 0.625^2], found by an exchange
-// algorithm in double precision; largest relative error 2.7e-6 with four coefficients (behind it stand probabilities of eight
-// bits) and 3.7e-9 with six (32-bit results).  Scores beyond, rare at the usual caps, take 1 - 2 / (1 + e^2|u|).
-constexpr float SH_TANH_MAX = 0.390625f;
+__device__ __forceinline__ float shaped_min3(float a, float b, float c) {
+  float y;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+
+// tanh u = u P(u^2): minimax polynomials of tanh(sqrt y) / sqrt y on [0, reach^2], found by an exchange algorithm in double precision.
+// Largest relative errors: three coefficients up to 0.35 2.8e-6, five up to 0.75 5.2e-7 (behind these two stand probabilities of eight bits);
+// four up to 0.35 3.4e-8, six up to 0.625 3.7e-9 (32-bit results).  Scores beyond, rare at the usual caps, take 1 - 2 / (1 + e^2|u|).
+constexpr float SH_TANH3_REACH = 0.35f, SH_TANH5_REACH = 0.75f, SH_TANH6_REACH = 0.625f;
 template <int N>
 __host__ __device__ constexpr float tanh_coef(int k) {
-  constexpr float c4[4] = {0.9999972581863403f, -0.333099901676178f, 0.13020624220371246f, -0.04011745750904083f};
+  constexpr float c3[3] = {0.9999971985816956f, -0.33291319012641907f, 0.1239800825715065f};
+  constexpr float c4[4] = {0.9999999403953552f, -0.3333243131637573f, 0.13296015560626984f, -0.04897000268101692f};
+  constexpr float c5[5] = {0.999999463558197f, -0.33328500390052795f, 0.13261182606220245f, -0.05011862516403198f, 0.012984894216060638f};
   constexpr float c6[6] = {1.0f, -0.3333326280117035f, 0.13331185281276703f, -0.0537252314388752f, 0.020603151991963387f, -0.005672425962984562f};
-  static_assert(N == 4 || N == 6, "four or six coefficients");
-  return N == 4 ? c4[k] : c6[k];
+  static_assert(N >= 3 && N <= 6, "three to six coefficients");
+  return N == 3 ? c3[k] : N == 4 ? c4[k] : N == 5 ? c5[k] : c6[k];
 }
 __device__ __forceinline__ float shaped_tanh_far(float u) {
   return copysignf(1.0f - __fdividef(2.0f, 1.0f + shaped_ex2(2.0f * SH_LOG2E * fabsf(u))), u);
 }
-// cap log2(e) tanh(x in) of one number
+// out tanh(x in) of one number
 __device__ __forceinline__ float shaped_cap(float x, float in, float out) {
   const float u = x * in, y = u * u;
   float t;
-  if (y > SH_TANH_MAX) {
+  if (!(y <= SH_TANH6_REACH * SH_TANH6_REACH)) {
     t = shaped_tanh_far(u);
   } else {
     t = tanh_coef<6>(5);
@@ -135,30 +160,29 @@ __device__ __forceinline__ float shaped_cap(float x, float in, float out) {
   }
   return t * out;
 }
-// the same of the 2 W numbers x, two at a time, N coefficients
-template <int N, int W>
-__device__ __forceinline__ void shaped_cap_pairs(uint64_t (&x)[W], float in, float out) {
-  const uint64_t in2 = f2_pair(in, in);
-  uint64_t u[W];
-  float top = 0.f;
+// out tanh(x in) + add of two numbers within reach.  With three or four coefficients the factors are folded into them (N + 1 operations a pair); the
+// powers of `in` stay in range of fp32 for in >= 2e-5, below that the reach is nothing.  With more, u is made first.
+template <int N>
+struct ShapedCapNear {
+  uint64_t c[N], in2;
+  float reach;
+  __device__ __forceinline__ ShapedCapNear(float in, float out, float in_out) {
+    float f = N <= 4 ? in_out : out;
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    u[i] = f2_mul(x[i], in2);
-    const uint64_t y = f2_mul(u[i], u[i]);
-    const float2 yy = f2_unpair(y);
-    top = shaped_max3(top, yy.x, yy.y);
-    uint64_t t = f2_pair(out * tanh_coef<N>(N - 1), out * tanh_coef<N>(N - 1));
-#pragma unroll
-    for (int k = N - 2; k >= 0; --k) t = f2_fma(t, y, f2_pair(out * tanh_coef<N>(k), out * tanh_coef<N>(k)));
-    x[i] = f2_mul(t, u[i]);
-  }
-  if (top > SH_TANH_MAX) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      const float2 uu = f2_unpair(u[i]), nn = f2_unpair(x[i]);
-      x[i] = f2_pair(uu.x * uu.x > SH_TANH_MAX ? out * shaped_tanh_far(uu.x) : nn.x, uu.y * uu.y > SH_TANH_MAX ? out * shaped_tanh_far(uu.y) : nn.y);
+    for (int k = 0; k < N; ++k) {
+      c[k] = f2_pair(f * tanh_coef<N>(k), f * tanh_coef<N>(k));
+      if (N <= 4) f *= in * in;
     }
+    in2 = f2_pair(in, in);
+    reach = N <= 4 ? (in >= 2e-5f ? SH_TANH3_REACH : -1.f) : N == 5 ? SH_TANH5_REACH : SH_TANH6_REACH;
   }
-}
+  __device__ __forceinline__ uint64_t operator()(uint64_t x, uint64_t add) const {
+    const uint64_t u = N <= 4 ? x : f2_mul(x, in2), y = f2_mul(u, u);
+    uint64_t t = f2_fma(c[N - 1], y, c[N - 2]);
+#pragma unroll
+    for (int k = N - 3; k >= 0; --k) t = f2_fma(t, y, c[k]);
+    return f2_fma(t, u, add);
+  }
+};
 
 }  // namespace smc

@@ -9,6 +9,8 @@
 //     sum                four warps per key tile: exp2(x - lse) of 128 columns, masked by the key's position where a column does not see all keys
 // What bounds it is the exponential, one per (token, head, key) pair; the product is half of the attention's.
 // The grid is persistent: key tiles of all sequences, those with most tokens behind them first.
+#include <type_traits>
+
 #include "shaped.cuh"
 
 namespace smc {
@@ -35,7 +37,7 @@ struct ShapedMassParams {
 // What a step's query rows bring along, by column
 struct alignas(16) MsColumns {
   float neg_lse[MS_Q], pos[MS_Q], first[MS_Q], last[MS_Q], slope[MS_Q];
-  float max_first[4], min_last[4];                    // over 32 columns each: a key between all of them is seen by every column
+  float max_first[4], min_last[4], min_pos4[4];       // over 32 columns each: a key between the first two is seen by every column
 };
 
 template <int D> struct MsShared {
@@ -246,7 +248,8 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         col.last[cl] = last;
         if (BIAS) col.slope[cl] = slope;
         const float mf = warp_max(first), ml = -warp_max(-last);
-        if (lane == 0) { col.max_first[lw] = mf; col.min_last[lw] = ml; }
+        const float mp = BIAS ? -warp_max(live ? -posf : -(float)SH_POS_END) : 0.f;
+        if (lane == 0) { col.max_first[lw] = mf; col.min_last[lw] = ml; col.min_pos4[lw] = mp; }
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.col_full[u % SLOTS]);
         const uint32_t dst0 = smem_u32(q_s + (size_t)st * TILE);
@@ -304,8 +307,9 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
       const int t = warp >> 2, r = (warp & 3) * 32 + lane, k = k0 + t * 128 + r;
       const uint32_t ts = tmem_base + (uint32_t)t * 256u + (((uint32_t)((warp & 3) * 32)) << 16);
       const float kpos = k < keys ? (float)pos_of(k) : -1.f;
-      const float mul = p.c.scale * SH_LOG2E, cap_in = CAP ? p.c.scale / p.c.cap : 0.f, cap_out = CAP ? p.c.cap * SH_LOG2E : 0.f;
+      const float mul = p.c.mul, cap_in = p.c.cap_in, cap_out = p.c.cap_out;
       const uint64_t mul2 = f2_pair(mul, mul), kpos2 = f2_pair(kpos, kpos);
+      const ShapedCapNear<4> near(cap_in, cap_out, mul);
       float total = 0.f;
       bool alive = true;
       for (int j = 0; j < n_steps; ++j) {
@@ -316,36 +320,64 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         tc_fence_after();
         const float4 mf = *reinterpret_cast<const float4*>(col.max_first), ml = *reinterpret_cast<const float4*>(col.min_last);
         const bool full = __all_sync(0xffffffffu, kpos >= fmaxf(fmaxf(mf.x, mf.y), fmaxf(mf.z, mf.w)) && kpos <= fminf(fminf(ml.x, ml.y), fminf(ml.z, ml.w)));
+        const float4 mp = *reinterpret_cast<const float4*>(col.min_pos4);
         uint64_t part[2] = {0ull, 0ull};              // a step's sum in four parts ahead of the running one: short chains of additions
+        const bool cause = !BIAS || __all_sync(0xffffffffu, kpos <= fminf(fminf(mp.x, mp.y), fminf(mp.z, mp.w)));     // every column lies behind this key
+        // exp2 of what `shaped` makes of pairs of scores and negated references
+        auto add_up = [&](const uint32_t (&w)[32], int c0, auto masked, auto shaped) {
 #pragma unroll
-        for (int c0 = 0; c0 < MS_Q; c0 += 32) {
-          uint32_t w[32];
-          tmem_ld_32x32b_x16(ts + buf * 128u + c0, *reinterpret_cast<uint32_t(*)[16]>(&w[0]));
-          tmem_ld_32x32b_x16(ts + buf * 128u + c0 + 16, *reinterpret_cast<uint32_t(*)[16]>(&w[16]));
-          tmem_ld_wait();
-          uint64_t x[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) x[i] = f2_pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-          if (CAP) {
-            shaped_cap_pairs<6, 8>(*reinterpret_cast<uint64_t(*)[8]>(&x[0]), cap_in, cap_out);
-            shaped_cap_pairs<6, 8>(*reinterpret_cast<uint64_t(*)[8]>(&x[8]), cap_in, cap_out);
-          }
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const uint64_t nl = *reinterpret_cast<const uint64_t*>(&col.neg_lse[c0 + 2 * i]);
-            x[i] = CAP ? f2_add(x[i], nl) : f2_fma(x[i], mul2, nl);
+          for (int i = 0; i < 32; i += 4) {
+            const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(&col.neg_lse[c0 + i]);
+            uint64_t off[2] = {nl.x, nl.y};
             if (BIAS) {
-              const float2 d = f2_unpair(f2_fma(*reinterpret_cast<const uint64_t*>(&col.pos[c0 + 2 * i]), f2_pair(-1.f, -1.f), kpos2));
-              x[i] = f2_fma(f2_pair(fabsf(d.x), fabsf(d.y)), *reinterpret_cast<const uint64_t*>(&col.slope[c0 + 2 * i]), x[i]);
+              const ulonglong2 at = *reinterpret_cast<const ulonglong2*>(&col.pos[c0 + i]), sl = *reinterpret_cast<const ulonglong2*>(&col.slope[c0 + i]);
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                uint64_t d = f2_fma(kpos2, f2_pair(-1.f, -1.f), k ? at.y : at.x);     // column less key
+                if (!cause) {
+                  const float2 v = f2_unpair(d);
+                  d = f2_pair(fabsf(v.x), fabsf(v.y));
+                }
+                off[k] = f2_fma(d, k ? sl.y : sl.x, off[k]);
+              }
             }
-            const float2 v = f2_unpair(x[i]);
-            float e0 = shaped_ex2(v.x), e1 = shaped_ex2(v.y);
-            if (!full) {
-              const int c = c0 + 2 * i;
-              e0 = kpos >= col.first[c] && kpos <= col.last[c] ? e0 : 0.f;
-              e1 = kpos >= col.first[c + 1] && kpos <= col.last[c + 1] ? e1 : 0.f;
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int c = c0 + i + 2 * k;
+              const float2 v = f2_unpair(shaped(f2_pair(__uint_as_float(w[i + 2 * k]), __uint_as_float(w[i + 2 * k + 1])), off[k]));
+              float e0 = shaped_ex2(v.x), e1 = shaped_ex2(v.y);
+              if constexpr (decltype(masked)::value) {
+                e0 = kpos >= col.first[c] && kpos <= col.last[c] ? e0 : 0.f;
+                e1 = kpos >= col.first[c + 1] && kpos <= col.last[c + 1] ? e1 : 0.f;
+              }
+              part[k] = f2_add(part[k], f2_pair(e0, e1));
             }
-            part[i & 1] = f2_add(part[i & 1], f2_pair(e0, e1));
+          }
+        };
+        auto number_by_number = [&](uint64_t x, uint64_t off) {
+          const float2 v = f2_unpair(x);
+          return f2_add(CAP ? f2_pair(shaped_cap(v.x, cap_in, cap_out), shaped_cap(v.y, cap_in, cap_out)) : f2_mul(x, mul2), off);
+        };
+#pragma unroll 1
+        for (int c0 = 0; c0 < MS_Q; c0 += 64) {
+          uint32_t w[2][32];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tmem_ld_32x32b_x16(ts + buf * 128u + c0 + 16 * k, *reinterpret_cast<uint32_t(*)[16]>(&w[k >> 1][(k & 1) * 16]));
+          tmem_ld_wait();
+          bool reach = true;
+          if (CAP) {
+            float far = 0.f;
+#pragma unroll
+            for (int i = 0; i < 64; i += 2) far = shaped_max3(far, fabsf(__uint_as_float(w[i >> 5][i & 31])), fabsf(__uint_as_float(w[i >> 5][(i & 31) + 1])));
+            reach = __all_sync(0xffffffffu, far * cap_in <= near.reach);
+          }
+          if (full && reach) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              add_up(w[h], c0 + 32 * h, std::false_type(), [&](uint64_t x, uint64_t off) { return CAP ? near(x, off) : f2_fma(x, mul2, off); });
+          } else {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) add_up(w[h], c0 + 32 * h, std::true_type(), number_by_number);
           }
         }
         tc_fence_before();
@@ -400,7 +432,7 @@ SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, i
   if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -162;
   if (mass_stride < bt_stride) return -163;
   ShapedMassParams p;
-  p.c = ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, scale, cap};
+  p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.runs = (const int4*)runs; p.lse = lse; p.mass = mass;
   p.ld_q = ld_q; p.mass_stride = mass_stride; p.n_runs = n_runs; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.pdl = pdl; p.status = status;
 #define SMC_SHAPED_MASS(DD)                                                                                            \

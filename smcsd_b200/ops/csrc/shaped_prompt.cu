@@ -25,6 +25,8 @@ template <> struct SpCfg<64> { static constexpr int NT = 2, BK = 128, SB = 1, UN
 template <> struct SpCfg<128> { static constexpr int NT = 2, BK = 128, SB = 1, UNITS = 5; };
 template <> struct SpCfg<256> { static constexpr int NT = 1, BK = 64, SB = 2, UNITS = 5; };
 
+constexpr float SP_NONE = -67108864.f;                // below any position, whatever is added
+
 struct ShapedPromptParams {
   ShapedCache c;
   const __nv_bfloat16* q;        // [T] rows of Hq * D, ld_q apart
@@ -40,8 +42,9 @@ struct ShapedPromptParams {
 
 template <int D> struct SpShared {
   static constexpr int SLOTS = SpCfg<D>::UNITS / 2 + 1;               // steps whose keys' positions are held
-  uint64_t kv_full[SpCfg<D>::UNITS], kv_empty[SpCfg<D>::UNITS], q_full[2], s_full[2][2], p_full[2][2], o_done[2][2], pos_full[SLOTS], turn[2][4];
-  alignas(16) float pos[SLOTS][SpCfg<D>::BK];
+  uint64_t kv_full[SpCfg<D>::UNITS], kv_empty[SpCfg<D>::UNITS], q_full[2], s_full[2][2], p_full[2][2][2], o_done[2][2], pos_full[SLOTS], turn[2][4];
+  alignas(16) float pos[SLOTS][SpCfg<D>::BK];         // of a step's keys, less that of the first; SP_NONE behind the last
+  float pos_first[SLOTS];
   uint32_t tmem_slot;
   int lo[8], hi[8], begin, end[2];
   volatile int abort;
@@ -131,12 +134,14 @@ template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__(SpCfg<D>::NT == 2 ? 512 : 384, 1)
 shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV) {
   constexpr int NT = SpCfg<D>::NT, UNITS = SpCfg<D>::UNITS, BK = SpCfg<D>::BK, SB = SpCfg<D>::SB;
+  constexpr int HALVES = BK / 64;                     // parts of a step's probabilities that are handed over on their own
   constexpr int KPW = BK / SP_LOADERS, KL = BK / 32;  // keys gathered by one loader warp; keys whose page a lane knows
   constexpr int NPAN = D / 64;                        // 64-element (128-byte) panels along the head dimension
   constexpr int PANEL_Q = 128 * 128, PANEL_KV = BK * 128;
   constexpr int Q_BYTES = NPAN * PANEL_Q, KV_BYTES = NPAN * PANEL_KV;
   constexpr int CPR = D / 8;                          // 16-byte chunks per row
   constexpr uint32_t COL_O = NT * SB * BK;            // tensor memory: scores (t * SB + buffer) * BK, probabilities over them, outputs behind
+  static_assert(COL_O + NT * D <= 512, "tensor memory");
   using Shared = SpShared<D>;
   constexpr int SLOTS = Shared::SLOTS;
   extern __shared__ uint8_t sp_smem_raw[];
@@ -170,7 +175,8 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
       for (int q = 0; q < 4; ++q) mbar_init(&S.turn[t][q], 1);
       for (int i = 0; i < SB; ++i) {
         mbar_init(&S.s_full[t][i], 1);
-        mbar_init(&S.p_full[t][i], 4);
+        mbar_init(&S.p_full[t][i][0], 4);
+        mbar_init(&S.p_full[t][i][1], 4);
         mbar_init(&S.o_done[t][i], 1);
       }
     }
@@ -231,18 +237,19 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
       atomicOr(p.status, SMC_ERR_BOUNDS);
       return 0;
     };
-    constexpr int LAG = UNITS - 2, PD = 2;            // gathered units in flight behind the newest; steps that page ids are read ahead
+    constexpr int LAG = UNITS - 2, PD = 2;           // gathered units in flight behind the newest; steps that page ids are read ahead
     int issued = 0;
     uint32_t gathered = 0;                            // bit (u & 31): this warp's part of unit u went through cp.async (arrival still owed)
-    int pg[PD][KL], pk[PD];
-    auto ahead = [&](int step, int (&ids)[KL], int& pos) {
+    int pg[PD][KL], pk[PD], p0[PD];
+    auto ahead = [&](int step, int (&ids)[KL], int& pos, int& first_pos) {
 #pragma unroll
       for (int i = 0; i < KL; ++i) ids[i] = step < n_steps ? bt[min(begin + step * BK + i * 32 + lane, end_all - 1)] : 0;
-      const int k = begin + step * BK + lw * KPW + lane;              // the positions this warp hands over
+      const int k = begin + step * BK + lw * KPW + lane, k0 = begin + step * BK;      // the positions this warp hands over
       pos = lane < KPW && k < end_all ? (kp != nullptr ? kp[k] : k) : -1;
+      first_pos = k0 < end_all ? (kp != nullptr ? kp[k0] : k0) : 0;
     };
 #pragma unroll
-    for (int d = 0; d < PD; ++d) ahead(d, pg[d], pk[d]);
+    for (int d = 0; d < PD; ++d) ahead(d, pg[d], pk[d], p0[d]);
     bool go = true;
     const uint64_t pol = l2_policy_evict_last();      // the other row tiles of this KV head read the same keys
     for (int j0 = 0; go && j0 < n_steps; j0 += PD) {
@@ -253,8 +260,8 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
         int page[KL];
 #pragma unroll
         for (int i = 0; i < KL; ++i) page[i] = checked(pg[d][i]);
-        const float pos = (float)pk[d];
-        ahead(j + PD, pg[d], pk[d]);
+        const float pos = pk[d] < 0 ? SP_NONE : (float)(pk[d] - p0[d]), pos_first = (float)p0[d];
+        ahead(j + PD, pg[d], pk[d], p0[d]);
         int base[KL / 2];
         bool rows_run[KL / 2];
 #pragma unroll
@@ -272,6 +279,7 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
           if (!__all_sync(0xffffffffu, ok)) { go = false; break; }
           if (kv == 0) {                              // the ring of positions turns with the keys
             if (lane < KPW) S.pos[j % SLOTS][lw * KPW + lane] = pos;
+            if (lw == 0 && lane == 0) S.pos_first[j % SLOTS] = pos_first;
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.pos_full[j % SLOTS]);
           }
@@ -355,12 +363,17 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
       bool ok = n == 0 || sp_wait(S, p.status, &S.q_full[t], 0);
       for (int j = 0; ok && j < min(n, SB); ++j) ok = issue_s(j);
       for (int j = 0; ok && j < n; ++j) {
-        if (!wait_unit(2 * j + 1) || !sp_wait(S, p.status, &S.p_full[t][j % SB], (uint32_t)(j / SB) & 1u)) { ok = false; break; }
-        tc_fence_after();
+        if (!wait_unit(2 * j + 1)) { ok = false; break; }
         const uint32_t v_addr = smem_u32(kv_s + (size_t)((2 * j + 1) % UNITS) * KV_BYTES);
 #pragma unroll
-        for (int k = 0; k < BK / 16; ++k)
-          sp_umma_ts(tO, tS + (uint32_t)(j % SB) * BK + 8 * k, umma_desc_mn_sw128(v_addr + k * 2048, PANEL_KV), idesc_o, (j | k) ? 1u : 0u);
+        for (int h = 0; h < HALVES; ++h) {            // the first half of the keys while the second takes its exponentials
+          if (!ok || !(ok = sp_wait(S, p.status, &S.p_full[t][j % SB][h], (uint32_t)(j / SB) & 1u))) break;
+          tc_fence_after();
+#pragma unroll
+          for (int k = h * 4; k < h * 4 + 4; ++k)
+            sp_umma_ts(tO, tS + (uint32_t)(j % SB) * BK + 8 * k, umma_desc_mn_sw128(v_addr + k * 2048, PANEL_KV), idesc_o, (j | k) ? 1u : 0u);
+        }
+        if (!ok) break;
         umma_commit(&S.o_done[t][j % SB]);            // O_t holds the sum over steps 0..j
         umma_commit(&S.kv_empty[(2 * j + 1) % UNITS]);
         if (j + SB < n) ok = issue_s(j + SB);
@@ -396,8 +409,9 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
     if (lane == 0) mbar_arrive(&S.q_full[t]);
     // rows behind the last token mask nothing, so that they do not send their warp the long way
     const float first_seen = live ? (float)see.x : 0.f, last_seen = live ? (float)see.y : (float)SH_POS_END;
-    const float mul = p.c.scale * SH_LOG2E, cap_in = CAP ? p.c.scale / p.c.cap : 0.f, cap_out = CAP ? p.c.cap * SH_LOG2E : 0.f;
+    const float mul = p.c.mul, cap_in = p.c.cap_in, cap_out = p.c.cap_out;
     const float slope = BIAS && live ? -p.c.slopes[hbase + r % G] * SH_LOG2E : 0.f;
+    const ShapedCapNear<3> near(cap_in, cap_out, mul);
     float m_ref = -INFINITY;                          // exponent reference of the row (log2 domain); -inf until it has seen a key
     uint64_t sum[2] = {0ull, 0ull};                   // its running sum, in four parts
     bool alive = true;
@@ -411,49 +425,48 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
 #pragma unroll
       for (int c0 = 0; c0 < BK; c0 += 16) tmem_ld_32x32b_x16(ts + c0, *reinterpret_cast<uint32_t(*)[16]>(&x[c0]));
       tmem_ld_wait();
-      auto pair = [&](int i) { return f2_pair(__uint_as_float(x[i]), __uint_as_float(x[i + 1])); };
-      auto put = [&](int i, uint64_t v) {
-        const float2 f = f2_unpair(v);
-        x[i] = __float_as_uint(f.x);
-        x[i + 1] = __float_as_uint(f.y);
-      };
-      if (CAP) {
+      auto val = [&](int i) { return __uint_as_float(x[i]); };
+      auto pair = [&](int i) { return f2_pair(val(i), val(i + 1)); };
+      // The shape of the scores is folded into the exponentials below: a tanh is monotone and a distance costs most at one end of the step, so the
+      // largest score and the distance of that end give a reference that no score exceeds, by no more than the step's scores differ.
+      float mx[2] = {-INFINITY, -INFINITY}, mn[2] = {INFINITY, INFINITY};
 #pragma unroll
-        for (int c0 = 0; c0 < BK; c0 += 16) {
-          uint64_t y[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = pair(c0 + 2 * i);
-          shaped_cap_pairs<4, 8>(y, cap_in, cap_out);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) put(c0 + 2 * i, y[i]);
+      for (int i = 0; i < BK; i += 4) {
+        mx[0] = shaped_max3(mx[0], val(i), val(i + 1));
+        mx[1] = shaped_max3(mx[1], val(i + 2), val(i + 3));
+        if (CAP || BIAS) {
+          mn[0] = shaped_min3(mn[0], val(i), val(i + 1));
+          mn[1] = shaped_min3(mn[1], val(i + 2), val(i + 3));
         }
       }
-      if (BIAS) {
-        const uint64_t sl = f2_pair(slope, slope), own = f2_pair(-pos_row, -pos_row), m2 = f2_pair(mul, mul);
-#pragma unroll
-        for (int i = 0; i < BK; i += 4) {
-          uint64_t at[2];                             // volatile: read where they are used, 128 scores leave no room for them all
-          asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(at[0]), "=l"(at[1]) : "r"(smem_u32(pos + i)));
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2 d = f2_unpair(f2_add(at[k], own));
-            const uint64_t away = f2_mul(f2_pair(fabsf(d.x), fabsf(d.y)), sl);
-            put(i + 2 * k, CAP ? f2_add(pair(i + 2 * k), away) : f2_fma(pair(i + 2 * k), m2, away));
-          }
-        }
-      }
+      const float most = fmaxf(mx[0], mx[1]), least = fminf(mn[0], mn[1]), reach = fmaxf(most, -least) * cap_in;
       // the keys of a step ascend, those behind the last (position -1) come at its end
-      const bool full = __all_sync(0xffffffffu, pos[0] >= first_seen && pos[BK - 1] >= 0.f && pos[BK - 1] <= last_seen);
-      if (!full) {
+      const float pos0 = S.pos_first[j % SLOTS], pos1 = pos0 + pos[BK - 1];
+      const bool full = __all_sync(0xffffffffu, pos0 >= first_seen && pos1 >= 0.f && pos1 <= last_seen);
+      // 0: scores as they are after this; 1: tanh by three coefficients (or none); 2: by five
+      int way = 1;
+      // (a row whose own position lies inside the step looks both ways)
+      if (!full || (BIAS && __any_sync(0xffffffffu, !((most - least) * mul < 60.f) || (pos0 < pos_row && pos1 > pos_row)))) way = 0;
+      else if (CAP && __any_sync(0xffffffffu, !(reach <= near.reach))) way = __any_sync(0xffffffffu, !(reach <= SH_TANH5_REACH)) ? 0 : 2;
+      float top;
+      if (way != 0) {
+        top = CAP ? shaped_cap(most, cap_in, cap_out) : most * mul;
+        if (BIAS) {
+          const float a = fabsf(pos0 - pos_row), b = fabsf(pos1 - pos_row);
+          top += slope * (slope > 0.f ? fmaxf(a, b) : fminf(a, b));
+        }
+      } else {
+        top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < BK; ++i)
-          if (!(pos[i] >= first_seen && pos[i] <= last_seen)) x[i] = 0xff800000u;        // -inf: probability zero
+        for (int i = 0; i < BK; ++i) {
+          float v = CAP ? shaped_cap(val(i), cap_in, cap_out) : val(i) * mul;
+          const float at = pos0 + pos[i];
+          if (BIAS) v = fmaf(fabsf(at - pos_row), slope, v);
+          if (!(at >= first_seen && at <= last_seen)) v = -INFINITY;                   // probability zero
+          x[i] = __float_as_uint(v);
+          top = fmaxf(top, v);
+        }
       }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int i = 0; i < BK; i += 2) mx[(i >> 1) & 3] = shaped_max3(mx[(i >> 1) & 3], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-      float top = fmaxf(shaped_max3(mx[0], mx[1], mx[2]), mx[3]);
-      if (!CAP && !BIAS) top *= mul;
       const bool grow = top > m_ref + 8.f;            // also true for the first visible key (m_ref = -inf)
       if (j >= 1 && __any_sync(0xffffffffu, grow)) {
         // rare after the first steps: PV of step j - 1 must have completed before O is rescaled in tensor memory
@@ -484,24 +497,46 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
                                : j == 0 || j > n_of[1] || sp_wait(S, p.status, &S.turn[0][q], (uint32_t)(j - 1) & 1u);
         if (!__all_sync(0xffffffffu, in_turn)) { alive = false; break; }
       }
-      const uint64_t mul2 = f2_pair(mul, mul), off = f2_pair(-ref, -ref);
+      // exp2 of what `shaped` makes of the pairs, 64 keys after the other
+      auto exponentials = [&](auto shaped) {
 #pragma unroll
-      for (int c0 = 0; c0 < BK; c0 += 32) {
-        uint32_t pk[16];
+        for (int h = 0; h < HALVES; ++h) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float2 e = f2_unpair(CAP || BIAS ? f2_add(pair(c0 + i), off) : f2_fma(pair(c0 + i), mul2, off));
-          const float p0 = shaped_ex2(e.x), p1 = shaped_ex2(e.y);
-          sum[(i >> 1) & 1] = f2_add(sum[(i >> 1) & 1], f2_pair(p0, p1));
-          pk[i >> 1] = sp_pack(p0, p1);
+          for (int c0 = h * 64; c0 < h * 64 + 64; c0 += 32) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int i = 0; i < 32; i += 2) {
+              const float2 e = f2_unpair(shaped(c0 + i));
+              const float p0 = shaped_ex2(e.x), p1 = shaped_ex2(e.y);
+              sum[(i >> 1) & 1] = f2_add(sum[(i >> 1) & 1], f2_pair(p0, p1));
+              pk[i >> 1] = sp_pack(p0, p1);
+            }
+            tmem_st_32x32b_x16(ts + (c0 >> 1), pk);
+          }
+          if (NT > 1 && h == HALVES - 1 && lane == 0) mbar_arrive(&S.turn[t ^ 1][warp & 3]);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&S.p_full[t][j % SB][h]);
         }
-        tmem_st_32x32b_x16(ts + (c0 >> 1), pk);
+      };
+      const uint64_t mul2 = f2_pair(mul, mul), off = f2_pair(-ref, -ref);
+      // distance's share less the reference: linear over the step, from its first key on
+      const float per = pos0 < pos_row ? -slope : slope, start = slope * fabsf(pos0 - pos_row) - ref;
+      const uint64_t per2 = f2_pair(per, per), start2 = f2_pair(start, start);
+      auto away = [&](int i) {
+        if (!BIAS) return off;
+        uint64_t at;                                  // volatile: read where it is used, the scores leave no room for all of them
+        asm volatile("ld.shared.b64 %0, [%1];" : "=l"(at) : "r"(smem_u32(pos + i)));
+        return f2_fma(at, per2, start2);
+      };
+      if (way == 0) exponentials([&](int i) { return f2_add(pair(i), off); });
+      else if (!CAP) exponentials([&](int i) { return f2_fma(pair(i), mul2, away(i)); });
+      else if (way == 1) exponentials([&](int i) { return near(pair(i), away(i)); });
+      else {
+        const ShapedCapNear<5> far(cap_in, cap_out, mul);
+        exponentials([&](int i) { return far(pair(i), away(i)); });
       }
-      if (NT > 1 && lane == 0) mbar_arrive(&S.turn[t ^ 1][warp & 3]);
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&S.p_full[t][j % SB]);
     }
     // the last product is done: read the accumulated O once
     if (alive && n > 0)
@@ -584,7 +619,7 @@ SMC_API int smc_shaped_prompt(const void* q, long long ld_q, const void* k_pool,
   if ((ld_q & 7) || (ld_out & 7) || (reinterpret_cast<uintptr_t>(bounds) & 7)) return -142;
   if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -143;
   ShapedPromptParams p;
-  p.c = ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, scale, cap};
+  p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.v_pool = (const __nv_bfloat16*)v_pool;
   p.runs = (const int4*)runs; p.out = (__nv_bfloat16*)out; p.lse = lse; p.ld_q = ld_q; p.ld_out = ld_out;
   p.n_runs = n_runs; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.pdl = pdl; p.status = status;

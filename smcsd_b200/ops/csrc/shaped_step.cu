@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
 
   if constexpr (D == 256 && Cfg::THREADS == 384) regs_more<ST_MANY>();
   const int mt = warp % MT, gi = warp / MT, kg = gi % Cfg::GW, turn = gi / Cfg::GW;  // row set, group; of it keys and turn
-  const float mul = p.c.scale * SH_LOG2E, cap_in = p.c.cap > 0.f ? p.c.scale / p.c.cap : 0.f, cap_out = p.c.cap * SH_LOG2E;
+  const float mul = p.c.mul, cap_in = p.c.cap_in, cap_out = p.c.cap_out;
   const int pitch = (M + 3) / 4 * 4;
   bool alive = true;
   int x = t_begin;
@@ -408,7 +408,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
           for (int i = 0; i < 4; ++i) {
             const float4 row = row_s[(mt * NQ + q) * 8 + 2 * c4 + (i & 1)];
             float v = sc[q][i] + sd[q][i];
-            v = p.c.cap > 0.f ? shaped_cap(v, cap_in, cap_out) : v * mul;
+            v = cap_in > 0.f ? shaped_cap(v, cap_in, cap_out) : v * mul;
             v = fmaf(row.w, fabsf(kp[i >> 1] - row.z), v);
             v = kp[i >> 1] >= row.x && kp[i >> 1] <= row.y ? v : -INFINITY;
             sc[q][i] = v;
@@ -758,7 +758,7 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
   if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hkv * ((E * (Hq / Hkv) + 3) / 4 * 4) * step_tile(D) * 4);       // the rest of it
   if (work_bytes < (long long)w.bytes || (mass != nullptr && w.score_tiles < 1)) return -154;
   ShapedStepParams p;
-  p.c = ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, scale, cap};
+  p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.v_pool = (const __nv_bfloat16*)v_pool;
   p.rows = rows; p.lens = lens; p.out = (__nv_bfloat16*)out; p.lse = lse; p.mass = mass;
   char* base = (char*)work;
