@@ -5,16 +5,20 @@
 // positions and weights, no key or value - into the same row, whose other tokens lose their references, or into another row, for which
 // references are taken.  Pages without a reference go on the free stack, the lowest on top, as the host's form leaves them.
 //
-// A cluster of eight blocks serves a row (one block alone a short one): blocks of 1024 tokens go round the cluster, so that one step
-// covers a run of the row and, with a barrier between its reads and its writes, compaction in place never overwrites what a later step reads.  The
-// n-th highest weight is found by three histograms of 11, 11 and 10 bits over order-preserving integers in shared memory, joined over the cluster.
-// What bounds it: 4 bytes per token and head read once, then barriers; the row that takes longest decides.
+// Two kernels.  The first finds out who stays: a cluster of eight blocks to a row (one block alone for a short one; rows with the same source share the
+// first one's answer), pieces of 512 tokens going round its blocks.  The n-th highest weight is found by three histograms of 11, 11 and 10 bits over
+// order-preserving integers in shared memory, joined over the cluster; a token's place is the number of tokens in front of it that stay, counted by
+// warps and joined over all pieces by one scan.  The second moves: a block to a row and head (or to its pages and positions), whose reads of a
+// run of places end before its writes, which lie in front of all later reads - so it may be the same row.
+// What bounds it: 4 bytes per token and head read once, then barriers and dependent reads; the row that takes longest decides.  (In one kernel, the moves of a cluster
+// kept in step by barriers between heads: 115 us for 16 rows of 65,000 tokens and 8 heads from two sources, %s now.)
 #include "common.cuh"
 
 namespace smc {
 
-constexpr int EV_CL = 8, EV_T = 1024, EV_BINS = 2048, EV_SOLO = 8192, EV_BLOCKS = 512;
-constexpr int EV_HEADS = 8;                            // heads moved between two barriers
+constexpr int EV_CL = 8, EV_T = 512, EV_BINS = 2048, EV_SOLO = 8192, EV_PIECES = 512;
+constexpr int EV_ENTRIES = 4096;                       // rows of a call
+constexpr int EV_MOVE = 8;                             // places of a thread between two barriers of the second kernel
 
 struct EvictParams {
   int* table;
@@ -23,13 +27,14 @@ struct EvictParams {
   int* lens;                                           // [rows]
   const int* src;
   const int* dst;
-  int* kept;                                           // [n_rows, keep] or null
+  int* kept;                                           // [n_rows, keep]
   int* refcount;
   int* free_stack;
   int* free_count;
   unsigned* done;                                      // workspace: blocks done, pages dead, a bit for every dead page; zero between calls
   unsigned* dead;
   unsigned* bits;
+  int* old;                                            // [EV_ENTRIES] what the second kernel has to know: the row's length before, -1: leave it alone
   long long bt_stride, kp_stride, mass_stride;
   int n_rows, rows, heads, n_pages, keep, first, last, capacity;
   int* status;
@@ -43,12 +48,12 @@ __device__ __forceinline__ unsigned ev_key(float f) {
 }
 
 struct EvShared {
-  unsigned hist[EV_BINS];
-  int eq[EV_BLOCKS / EV_CL], sure[EV_BLOCKS / EV_CL];   // of this block's pieces: ties with the border, tokens that stay anyhow
-  int eq_at[EV_BLOCKS / EV_CL], kept_at[EV_BLOCKS / EV_CL];
-  int warp[32], warp2[32];
+  alignas(16) unsigned hist[EV_BINS], total[2][EV_BINS];           // of this block; of the cluster, in its first block, for every other pass
+  int eq_of[EV_PIECES / EV_CL][EV_T / 32], sure_of[EV_PIECES / EV_CL][EV_T / 32];     // of a piece's warps: ties with the border, tokens that stay anyhow; then those ahead
+  int eq[EV_PIECES / EV_CL], sure[EV_PIECES / EV_CL];   // of this block's pieces; then those ahead
+  int warp[32];
   unsigned digit;
-  int left, total;
+  int left, last;
 };
 
 // exclusive sum of v over the block; every thread also gets the whole sum
@@ -62,14 +67,18 @@ __device__ __forceinline__ int ev_scan(int v, int* warp_sum, int& all) {
   }
   if (lane == 31) warp_sum[warp] = sum;
   __syncthreads();
-  const int mine = warp_sum[lane];
+  const int mine = lane < EV_T / 32 ? warp_sum[lane] : 0;
   const int ahead = __reduce_add_sync(0xffffffffu, lane < warp ? mine : 0);
   all = __reduce_add_sync(0xffffffffu, mine);
   __syncthreads();
   return ahead + sum - v;
 }
+// add to a word of the cluster's first block
+__device__ __forceinline__ void ev_add_first(unsigned* word, unsigned v) {
+  asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(dsmem_map(smem_u32(word), 0)), "r"(v) : "memory");
+}
 
-__global__ void __launch_bounds__(EV_T, 1) evict_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(EV_T, 2) evict_kernel(const EvictParams p) {
   extern __shared__ unsigned ev_keys[];                // [capacity]: piece i of this block at i * EV_T
   __shared__ EvShared S;
   const int t = threadIdx.x, rank = (int)cluster_ctarank(), b = blockIdx.x / EV_CL;
@@ -79,15 +88,20 @@ __global__ void __launch_bounds__(EV_T, 1) evict_kernel(const EvictParams p) {
   bool clash = false;
   for (int o = t; o < p.n_rows; o += EV_T)
     if (o != b) clash |= p.dst[o] == dst || p.dst[o] == src || p.src[o] == dst;
-  fine = !__syncthreads_or(clash) && fine;
-  const int n = fine ? p.lens[src] : 0, old = fine ? p.lens[dst] : 0;
-  fine = fine && n >= 0 && n <= p.bt_stride && old >= 0 && old <= p.bt_stride;
+  fine = !__syncthreads_or(clash) && fine;             // (a value known to the whole cluster: every block asks the same)
+  bool shared = false;                                 // an earlier entry has the same source: its answer serves
+  for (int o = t; o < b; o += EV_T) shared |= p.src[o] == src;
+  shared = __syncthreads_or(shared);
+  int n = src >= 0 && src < p.rows ? p.lens[src] : -1;
+  const int old = fine ? p.lens[dst] : 0;
+  const bool known = n >= 0 && n <= p.bt_stride;       // (an entry that clashes still answers for those that share its source)
+  n = known ? n : 0;
+  fine = fine && known && old >= 0 && old <= p.bt_stride;
   const bool solo = n <= EV_SOLO, in_place = src == dst;
   const int CL = solo ? 1 : EV_CL;
   auto barrier = [&] { if (solo) __syncthreads(); else cluster_sync(); };
-  const bool idle = solo && rank > 0;
   if (!fine && rank == 0 && t == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
-  if (fine && !idle) {
+  if (known && !shared && !(solo && rank > 0)) {
     const int pieces = (n + EV_T - 1) / EV_T, steps = (pieces + CL - 1) / CL;
     const bool all = n <= p.keep;
     const int m = min(n, p.keep), lo = p.first, hi = n - p.last, want = p.keep - p.first - p.last;      // want of [lo, hi) stay
@@ -95,52 +109,75 @@ __global__ void __launch_bounds__(EV_T, 1) evict_kernel(const EvictParams p) {
     unsigned border = 0;
     int need = 0;                                      // tokens at the border that stay
     if (!all) {
-      for (int i = 0; i < steps; ++i) {
-        const int idx = index(i);
-        if (idx < n) {
-          const float* w = p.mass + (size_t)src * p.heads * p.mass_stride + idx;
-          float sum = w[0];
-#pragma unroll 8
-          for (int h = 1; h < p.heads; ++h) sum += w[(size_t)h * p.mass_stride];
-          ev_keys[i * EV_T + t] = ev_key(sum);
+      for (int i0 = 0; i0 < steps; i0 += 4) {          // 32 reads of a thread in flight
+        float sum[4];
+        for (int h0 = 0; h0 < p.heads; h0 += 8) {
+          float w[4][8];
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int h = 0; h < 8; ++h) {
+              const int idx = index(i0 + u);
+              w[u][h] = idx < n && h0 + h < p.heads ? p.mass[((size_t)src * p.heads + h0 + h) * p.mass_stride + idx] : 0.f;
+            }
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int h = 0; h < 8; ++h)
+              if (h0 + h < p.heads) sum[u] = h0 + h == 0 ? w[u][h] : sum[u] + w[u][h];
         }
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (index(i0 + u) < n) ev_keys[(i0 + u) * EV_T + t] = ev_key(sum[u]);
       }
       need = want;
       if (want > 0) {
         int shift = 32;
+        for (int i = t; i < EV_BINS; i += EV_T) S.total[0][i] = 0;
         for (int pass = 0; pass < 3; ++pass) {
           const int bits = pass < 2 ? 11 : 10;
           const unsigned known = shift < 32 ? border >> shift : 0u;
-          for (int i = t; i < EV_BINS; i += EV_T) S.hist[i] = 0;
+          unsigned* hist = solo ? S.total[pass & 1] : S.hist;
+          if (!solo)
+            for (int i = t; i < EV_BINS; i += EV_T) S.hist[i] = 0;
           __syncthreads();
           for (int i = 0; i < steps; ++i) {
             const int idx = index(i);
-            if (idx >= lo && idx < hi) {
-              const unsigned k = ev_keys[i * EV_T + t];
-              if (shift == 32 || k >> shift == known) atomicAdd(&S.hist[k >> (shift - bits) & ((1u << bits) - 1u)], 1u);
+            const unsigned k = idx >= lo && idx < hi ? ev_keys[i * EV_T + t] : 0u;
+            const bool counts = idx >= lo && idx < hi && (shift == 32 || k >> shift == known);
+            const unsigned digit = k >> (shift - bits) & ((1u << bits) - 1u);
+            if (pass == 0) {                           // most tokens share a few exponents: one addition for all lanes of a digit
+              const unsigned same = __match_any_sync(0xffffffffu, counts ? digit : 0xffffffffu);
+              if (counts && (threadIdx.x & 31) == __ffs(same) - 1) atomicAdd(&hist[digit], (unsigned)__popc(same));
+            } else if (counts) {
+              atomicAdd(&hist[digit], 1u);
             }
           }
           barrier();
-          // two bins a thread, the highest first, over all blocks of the cluster
-          int count[2] = {0, 0};
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int bin = EV_BINS - 1 - (2 * t + i);
-            if (solo) count[i] = (int)S.hist[bin];
-            else
-              for (int c = 0; c < EV_CL; ++c) count[i] += (int)ld_dsmem_u32(smem_u32(&S.hist[bin]), c);
+          if (!solo)
+            for (int i = t; i < EV_BINS; i += EV_T)
+              if (S.hist[i] != 0u) ev_add_first(&S.total[pass & 1][i], S.hist[i]);
+          for (int i = t; i < EV_BINS; i += EV_T) S.total[(pass & 1) ^ 1][i] = 0;
+          barrier();
+          // four bins a thread, the highest first
+          constexpr int B = EV_BINS / EV_T;
+          int count[B], mine = 0;
+          static_assert(B == 4, "a thread's bins are read at once");
+          {
+            const uint32_t at = dsmem_map(smem_u32(&S.total[pass & 1][EV_BINS - 4 - 4 * t]), solo ? cluster_ctarank() : 0);
+            asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(count[3]), "=r"(count[2]), "=r"(count[1]), "=r"(count[0]) : "r"(at) : "memory");
+            mine = count[0] + count[1] + count[2] + count[3];
           }
-          int sum;
-          const int ahead = ev_scan(count[0] + count[1], S.warp, sum);
+          int sum, before = ev_scan(mine, S.warp, sum);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const int before = ahead + (i ? count[0] : 0);
+          for (int i = 0; i < B; ++i) {
             if (before < need && need <= before + count[i]) {
-              S.digit = (unsigned)(EV_BINS - 1 - (2 * t + i));
+              S.digit = (unsigned)(EV_BINS - 1 - (B * t + i));
               S.left = need - before;
             }
+            before += count[i];
           }
-          barrier();                                   // the histograms are read, the digit is there
+          __syncthreads();
           shift -= bits;
           border |= S.digit << shift;
           need = S.left;
@@ -158,95 +195,80 @@ __global__ void __launch_bounds__(EV_T, 1) evict_kernel(const EvictParams p) {
       sure = idx < n && (all || !inner || (want > 0 && k > border));
       tie = idx < n && !all && inner && k == border;
     };
+    const int warp = t >> 5, lane = t & 31;
+    const unsigned below = (1u << lane) - 1u;
     for (int i = 0; i < steps; ++i) {
       bool sure, tie;
       flags(i, sure, tie);
-      const int a = __syncthreads_count(sure), e = __syncthreads_count(tie);
-      if (t == 0) { S.sure[i] = a; S.eq[i] = e; }
+      const unsigned a = __ballot_sync(0xffffffffu, sure), e = __ballot_sync(0xffffffffu, tie);
+      if (lane == 0) { S.sure_of[i][warp] = __popc(a); S.eq_of[i][warp] = __popc(e); }
+    }
+    __syncthreads();
+    if (t < steps) {                                   // warps of a piece -> those ahead of each
+      int a = 0, e = 0;
+#pragma unroll
+      for (int w = 0; w < EV_T / 32; ++w) {
+        const int wa = S.sure_of[t][w], we = S.eq_of[t][w];
+        S.sure_of[t][w] = a;
+        S.eq_of[t][w] = e;
+        a += wa;
+        e += we;
+      }
+      S.sure[t] = a;
+      S.eq[t] = e;
     }
     barrier();
-    {
-      int sure = 0, eq = 0, all_eq, all_kept;
+    {                                                  // pieces of the row -> those ahead of each
+      int sure = 0, eq = 0, sum;
       if (t < pieces) {
-        const int c = t % CL, i = t / CL;
-        sure = solo ? S.sure[i] : (int)ld_dsmem_u32(smem_u32(&S.sure[i]), c);
-        eq = solo ? S.eq[i] : (int)ld_dsmem_u32(smem_u32(&S.eq[i]), c);
+        sure = solo ? S.sure[t] : (int)ld_dsmem_u32(smem_u32(&S.sure[t / CL]), t % CL);
+        eq = solo ? S.eq[t] : (int)ld_dsmem_u32(smem_u32(&S.eq[t / CL]), t % CL);
       }
-      const int eq_at = ev_scan(eq, S.warp, all_eq);
-      const int kept_at = ev_scan(sure + max(0, min(eq, need - eq_at)), S.warp2, all_kept);
-      if (t < pieces && t % CL == rank) { S.eq_at[t / CL] = eq_at; S.kept_at[t / CL] = kept_at; }
+      const int sure_at = ev_scan(sure, S.warp, sum), eq_at = ev_scan(eq, S.warp, sum);
+      barrier();                                       // all blocks have read the counts
+      if (t < pieces && t % CL == rank) { S.sure[t / CL] = sure_at; S.eq[t / CL] = eq_at; }
       __syncthreads();
     }
     for (int i = 0; i < steps; ++i) {
+      const int idx = index(i);
       bool sure, tie;
       flags(i, sure, tie);
-      const int idx = index(i);
-      const bool mine = i * CL + rank < pieces;        // uniform over the block
-      int sum, at = 0;
-      bool stay = false;
-      if (mine) {
-        const int eq_at = S.eq_at[i] + ev_scan(tie, S.warp, sum);
-        stay = sure || (tie && eq_at < need);
-        at = S.kept_at[i] + ev_scan(stay, S.warp2, sum);
-        if (stay && p.kept != nullptr) p.kept[(size_t)b * p.keep + at] = idx;
-      }
-      if (all && in_place) continue;                   // nothing moves
-      int page = 0, pos = 0;
-      if (mine && idx < n) {
-        page = p.table[(size_t)src * p.bt_stride + idx];
-        if (p.key_pos != nullptr) pos = p.key_pos[(size_t)src * p.kp_stride + idx];
+      const unsigned a = __ballot_sync(0xffffffffu, sure), e = __ballot_sync(0xffffffffu, tie);
+      // in front of a token stay the sure ones and the first `need` ties
+      const int eq = S.eq[i] + S.eq_of[i][warp] + __popc(e & below);
+      if (sure || (tie && eq < need)) {
+        p.kept[(size_t)b * p.keep + S.sure[i] + S.sure_of[i][warp] + __popc(a & below) + min(eq, need)] = idx;
+      } else if (fine && in_place && idx < n) {        // it leaves the row
+        const int page = p.table[(size_t)src * p.bt_stride + idx];
         if (page < 0 || page > p.n_pages) {
           atomicOr(p.status, SMC_ERR_BOUNDS);
         } else if (page > 0) {
-          if (in_place && !stay) {
-            const int before = atomicSub(&p.refcount[page], 1);
-            if (before == 1) {
-              atomicOr(&p.bits[page >> 5], 1u << (page & 31));
-              atomicAdd(p.dead, 1u);
-            } else if (before < 1) {
-              atomicAdd(&p.refcount[page], 1);         // nobody held it
-            }
-          } else if (!in_place && stay) {
-            atomicAdd(&p.refcount[page], 1);
+          const int before = atomicSub(&p.refcount[page], 1);
+          if (before == 1) {
+            atomicOr(&p.bits[page >> 5], 1u << (page & 31));
+            atomicAdd(p.dead, 1u);
+          } else if (before < 1) {
+            atomicAdd(&p.refcount[page], 1);           // nobody held it
           }
-        }
-      }
-      for (int h0 = 0; h0 < p.heads; h0 += EV_HEADS) {
-        float w[EV_HEADS];
-#pragma unroll
-        for (int h = 0; h < EV_HEADS; ++h)
-          if (stay && h0 + h < p.heads) w[h] = p.mass[((size_t)src * p.heads + h0 + h) * p.mass_stride + idx];
-        if (in_place) barrier();
-        if (stay) {
-          if (h0 == 0) {
-            p.table[(size_t)dst * p.bt_stride + at] = page;
-            if (p.key_pos != nullptr) p.key_pos[(size_t)dst * p.kp_stride + at] = pos;
-          }
-#pragma unroll
-          for (int h = 0; h < EV_HEADS; ++h)
-            if (h0 + h < p.heads) p.mass[((size_t)dst * p.heads + h0 + h) * p.mass_stride + at] = w[h];
         }
       }
     }
-    if (in_place) barrier();                           // everything has been read
-    // behind the kept tokens: no weight up to the row's old length, no index
-    const int step = CL * EV_T, t0 = rank * EV_T + t;
-    for (int h = 0; h < p.heads; ++h)
-      for (int i = m + t0; i < old; i += step) p.mass[((size_t)dst * p.heads + h) * p.mass_stride + i] = 0.f;
-    if (p.kept != nullptr)
-      for (int i = m + t0; i < p.keep; i += step) p.kept[(size_t)b * p.keep + i] = -1;
-    barrier();                                         // all blocks have read the lengths, and no block leaves while its counts are read
-    if (rank == 0 && t == 0) p.lens[dst] = m;
+    for (int i = m + rank * EV_T + t; i < p.keep; i += CL * EV_T) p.kept[(size_t)b * p.keep + i] = -1;
+    barrier();                                         // no block leaves while its counts are read, and all have read the lengths
+  }
+  if (rank == 0 && t == 0) {
+    p.old[b] = fine ? old : -1;
+    if (fine) p.lens[dst] = min(n, p.keep);
   }
   // the block that comes last puts dead pages on the free stack
   __syncthreads();
   if (t == 0) {
     __threadfence();
-    S.total = atomicAdd(p.done, 1u) == gridDim.x - 1;
+    S.last = atomicAdd(p.done, 1u) == gridDim.x - 1;
     __threadfence();
   }
   __syncthreads();
-  if (!S.total) return;
+  if (!S.last) return;
   if (t == 0) {
     S.left = (int)atomicAdd(p.dead, 0u);
     *p.done = 0;
@@ -277,25 +299,80 @@ __global__ void __launch_bounds__(EV_T, 1) evict_kernel(const EvictParams p) {
   if (t == 0) *p.free_count = min(base + sum, p.n_pages);
 }
 
+// Part 0 of an entry: pages with their references, positions, the list of an entry that shares another one's answer; part 1 + h: the weights of a head.
+__global__ void __launch_bounds__(EV_T) evict_move_kernel(const EvictParams p) {
+  const int t = threadIdx.x, b = blockIdx.x / (p.heads + 1), part = blockIdx.x % (p.heads + 1) - 1;
+  const int src = p.src[b], dst = p.dst[b];
+  int leader = b;
+  for (int o = t; o < b; o += EV_T)
+    if (p.src[o] == src) { leader = o; break; }
+  __shared__ int s_leader;
+  if (t == 0) s_leader = b;
+  __syncthreads();
+  if (leader < b) atomicMin(&s_leader, leader);
+  __syncthreads();
+  leader = s_leader;
+  pdl_wait_prior_grid();
+  const int old = p.old[b];
+  if (old < 0) return;
+  const int m = p.lens[dst];
+  const int* list = p.kept + (size_t)leader * p.keep;
+  // every thread EV_MOVE places of a run; between its reads and its writes a barrier where the row is its own source
+  auto move = [&](auto* from, auto* to, auto also) {
+    for (int p0 = 0; p0 < m; p0 += EV_T * EV_MOVE) {
+      int idx[EV_MOVE];
+      decltype(*from + 0) v[EV_MOVE];
+#pragma unroll
+      for (int u = 0; u < EV_MOVE; ++u) idx[u] = p0 + u * EV_T + t < m ? list[p0 + u * EV_T + t] : -1;
+#pragma unroll
+      for (int u = 0; u < EV_MOVE; ++u)
+        if (idx[u] >= 0) v[u] = from[idx[u]];
+      if (src == dst) __syncthreads();
+#pragma unroll
+      for (int u = 0; u < EV_MOVE; ++u)
+        if (idx[u] >= 0) {
+          to[p0 + u * EV_T + t] = v[u];
+          also(p0 + u * EV_T + t, idx[u], v[u]);
+        }
+    }
+  };
+  if (part < 0) {
+    move(p.table + (size_t)src * p.bt_stride, p.table + (size_t)dst * p.bt_stride, [&](int at, int idx, int page) {
+      if (page < 0 || page > p.n_pages) atomicOr(p.status, SMC_ERR_BOUNDS);
+      else if (page > 0 && src != dst) atomicAdd(&p.refcount[page], 1);
+      if (leader != b) p.kept[(size_t)b * p.keep + at] = idx;
+    });
+    if (p.key_pos != nullptr)
+      move(p.key_pos + (size_t)src * p.kp_stride, p.key_pos + (size_t)dst * p.kp_stride, [](int, int, int) {});
+    if (leader != b)
+      for (int i = m + t; i < p.keep; i += EV_T) p.kept[(size_t)b * p.keep + i] = -1;
+  } else {
+    float* to = p.mass + ((size_t)dst * p.heads + part) * p.mass_stride;
+    move(p.mass + ((size_t)src * p.heads + part) * p.mass_stride, to, [](int, int, float) {});
+    __syncthreads();
+    for (int i = m + t; i < old; i += EV_T) to[i] = 0.f;              // no weight behind the kept tokens, up to the row's old length
+  }
+}
+
 }  // namespace smc
 
 // Bytes of workspace (zeros at first) for an allocator of n_pages pages.
-SMC_API long long smc_evict_work(int n_pages) { return n_pages < 1 ? -1 : 256 + ((long long)n_pages / 32 + 1) * 4; }
+SMC_API long long smc_evict_work(int n_pages) { return n_pages < 1 ? -1 : 256 + smc::EV_ENTRIES * 4 + ((long long)n_pages / 32 + 1) * 4; }
 
 // src, dst [n_rows] int32 rows of table [rows, bt_stride], key_pos [rows, kp_stride] or null and mass [rows, heads, mass_stride] fp32, with lens [rows]; a
-// row is written by one entry at most and then read by no other.  kept [n_rows, keep] or null.
+// row is written by one entry at most and then read by no other.  kept [n_rows, keep].
 SMC_API int smc_evict(int* table, long long bt_stride, int* key_pos, long long kp_stride, float* mass, long long mass_stride, int* lens, int rows,
                       const int* src, const int* dst, int n_rows, int heads, int keep, int first, int last, int* kept, int* refcount, int* free_stack,
                       int* free_count, int n_pages, void* work, long long work_bytes, int* status, cudaStream_t st) {
   using namespace smc;
   if (n_rows <= 0) return 0;
-  if (heads < 1 || keep < 1 || first < 0 || last < 0 || first > keep || last > keep - first) return -170;
-  if (bt_stride < 1 || bt_stride > EV_BLOCKS * EV_T / 2 || mass_stride < bt_stride || (key_pos != nullptr && kp_stride < bt_stride)) return -171;
+  if (n_rows > EV_ENTRIES || kept == nullptr || heads < 1 || keep < 1 || first < 0 || last < 0 || first > keep || last > keep - first) return -170;
+  if (bt_stride < 1 || bt_stride > (long long)EV_PIECES * EV_T || mass_stride < bt_stride || (key_pos != nullptr && kp_stride < bt_stride)) return -171;
   if (work_bytes < smc_evict_work(n_pages) || (reinterpret_cast<uintptr_t>(work) & 3)) return -172;
   EvictParams p;
   p.table = table; p.key_pos = key_pos; p.mass = mass; p.lens = lens; p.src = src; p.dst = dst; p.kept = kept;
   p.refcount = refcount; p.free_stack = free_stack; p.free_count = free_count;
-  p.done = (unsigned*)work; p.dead = p.done + 1; p.bits = p.done + 64;
+  p.done = (unsigned*)work; p.dead = p.done + 1; p.old = (int*)(p.done + 64); p.bits = p.done + 64 + EV_ENTRIES;
   p.bt_stride = bt_stride; p.kp_stride = kp_stride; p.mass_stride = mass_stride;
   p.n_rows = n_rows; p.rows = rows; p.heads = heads; p.n_pages = n_pages; p.keep = keep; p.first = first; p.last = last; p.status = status;
   const long long per = (bt_stride + EV_CL * EV_T - 1) / (EV_CL * EV_T) * EV_T, alone = (bt_stride < EV_SOLO ? (bt_stride + EV_T - 1) / EV_T * EV_T : EV_SOLO);
@@ -314,5 +391,11 @@ SMC_API int smc_evict(int* table, long long bt_stride, int* key_pos, long long k
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, evict_kernel, p));
+  // (rows and lists that the second kernel reads ahead of its wait are the caller's: the first kernel lets it start at its end only)
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)(n_rows * (heads + 1)));
+  cfg.dynamicSmemBytes = 0;
+  CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, evict_move_kernel, p));
   return 0;
 }

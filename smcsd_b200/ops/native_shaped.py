@@ -186,8 +186,8 @@ def evict_work_bytes(n_pages: int) -> int:
 
 
 def evict_tokens(block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, lens: torch.Tensor, mass: torch.Tensor, refcount: torch.Tensor,
-                 free_stack: torch.Tensor, free_count: torch.Tensor, *, keep: int, first: int, last: int, work: torch.Tensor, status: torch.Tensor,
-                 key_pos: Optional[torch.Tensor] = None, kept: Optional[torch.Tensor] = None) -> None:
+                 free_stack: torch.Tensor, free_count: torch.Tensor, *, keep: int, first: int, last: int, kept: torch.Tensor, work: torch.Tensor,
+                 status: torch.Tensor, key_pos: Optional[torch.Tensor] = None) -> None:
     """Of the ``lens[row]`` tokens of each row in ``src`` [n] the first ``first``, the last ``last`` and those between with the highest sum of ``mass`` over the KV
     heads stay, at most ``keep`` in all (equal sums: the lower index).  They move, in their order, with page, position and weights to the row
     in ``dst``: the same one, whose other tokens give up their pages' references, or another, free one, which takes references.  ``lens`` [rows]
@@ -205,7 +205,7 @@ def evict_tokens(block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor
     if free_stack.shape[0] < pages:
         raise ValueError(f"free_stack: room for {pages} pages expected, got {free_stack.shape[0]}")
     K._check(L.smc_evict(bt, bts if R > 1 else cols, kp, kps if R > 1 else max(kps, cols), mp, ms, _is(lens, "lens", _I32, dev, (R,)), R, _is(src, "src", _I32, dev, (n,)),
-                         _is(dst, "dst", _I32, dev, (n,)), n, mass.shape[1], keep, first, last, None if kept is None else _is(kept, "kept", _I32, dev, (n, keep)),
+                         _is(dst, "dst", _I32, dev, (n,)), n, mass.shape[1], keep, first, last, _is(kept, "kept", _I32, dev, (n, keep)),
                          _is(refcount, "refcount", _I32, dev, refcount.shape), _is(free_stack, "free_stack", _I32, dev, free_stack.shape),
                          _is(free_count, "free_count", _I32, dev, free_count.shape), pages, _is(work, "work", _U8, dev, work.shape), work.numel(),
                          _is(status, "status", _I32, dev), K._stream()), "smc_evict")
