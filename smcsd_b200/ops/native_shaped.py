@@ -45,63 +45,70 @@ def _library():
         for name in ("smc_shaped_prompt", "smc_shaped_step", "smc_shaped_mass", "smc_evict"):
             getattr(L, name).restype = i
         L.smc_shaped_step_work.restype = L.smc_evict_work.restype = ll
+        K._KERNELS_PER_CALL.update({"smc_evict": 2, "smc_shaped_step with mass": 2})
         _lib = L
     return _lib
 
 
-def _is(t: torch.Tensor, name: str, dtype: torch.dtype, device, shape=None) -> int:
-    """Address of a tensor of this type on this device whose last axis is contiguous; ``shape``: at least these sizes, all axes contiguous."""
-    if t.dtype is not dtype or t.device != device:
-        raise ValueError(f"{name}: {dtype} on {device} expected, got {t.dtype} on {t.device}")
-    if shape is not None:
-        if t.dim() != len(shape) or not t.is_contiguous() or any(a < b for a, b in zip(t.shape, shape)) or t.shape[1:] != shape[1:]:
-            raise ValueError(f"{name}: contiguous {tuple(shape)} expected, got {tuple(t.shape)} with strides {t.stride()}")
-    elif t.stride(-1) != 1 and t.shape[-1] > 1:
-        raise ValueError(f"{name}: the last axis has to be contiguous, got strides {t.stride()}")
+def _wrong(t: torch.Tensor, name: str, want: str):
+    return ValueError(f"{name}: {want} expected, got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
+
+
+def _flat(t: torch.Tensor, name: str, dtype: torch.dtype, dev: int, shape) -> int:
+    """Address of a contiguous tensor of this type on this device, at least ``shape[0]`` long and of those further sizes."""
+    got = t.shape
+    if t.dtype is not dtype or t.get_device() != dev or len(got) != len(shape) or got[0] < shape[0] or got[1:] != shape[1:] or not t.is_contiguous():
+        raise _wrong(t, name, f"contiguous {dtype} {tuple(shape)} on cuda:{dev}")
     return t.data_ptr()
 
 
-def _table(t: Optional[torch.Tensor], name: str, device, rows: int, cols: int):
-    """Address and row stride of an int32 table of at least ``rows`` x ``cols``, or nothing."""
-    if t is None:
-        return None, 0
-    p = _is(t, name, _I32, device)
-    if t.dim() != 2 or t.shape[0] < rows or t.shape[1] < cols:
-        raise ValueError(f"{name}: at least [{rows}, {cols}] expected, got {tuple(t.shape)}")
-    return p, t.stride(0)
+def _device(q: torch.Tensor) -> int:
+    dev = q.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors on the current CUDA device expected, got {q.device}")
+    return dev
 
 
-def _device(q: torch.Tensor):
-    device = q.device
-    if device.type != "cuda" or device.index != torch._C._cuda_getDevice():
-        raise ValueError(f"tensors on the current CUDA device expected, got {device}")
-    return device
+def _rows(t: torch.Tensor, name: str, dev: int, T: int, width: int):
+    """Address and stride of at least T rows of ``width`` bf16 values."""
+    got, stride = t.shape, t.stride()
+    if t.dtype is not _BF16 or t.get_device() != dev or len(got) != 2 or got[0] < T or got[1] != width or stride[1] != 1:
+        raise _wrong(t, name, f"at least {T} rows of {width} bfloat16 values on cuda:{dev}")
+    return t.data_ptr(), stride[0]
 
 
-def _rows(t: torch.Tensor, name: str, device, T: int, width: int):
-    """Address and stride of T rows of ``width`` bf16 values."""
-    p = _is(t, name, _BF16, device)
-    if t.dim() != 2 or t.shape[0] < T or t.shape[1] != width:
-        raise ValueError(f"{name}: at least [{T}, {width}] expected, got {tuple(t.shape)}")
-    return p, t.stride(0)
+def _pool(t: torch.Tensor, name: str, dev: int, width: int) -> int:
+    if t.dtype is not _BF16 or t.get_device() != dev or t.dim() != 2 or t.shape[1] != width or not t.is_contiguous():
+        raise _wrong(t, name, f"contiguous bfloat16 [pages + 1, {width}] on cuda:{dev}")
+    return t.data_ptr()
 
 
-def _pool(t: torch.Tensor, name: str, device, width: int) -> int:
-    if t.dim() != 2 or t.shape[1] != width:
-        raise ValueError(f"{name}: [pages + 1, {width}] expected, got {tuple(t.shape)}")
-    return _is(t, name, _BF16, device, t.shape)
+def _tables(block_table: torch.Tensor, key_pos: Optional[torch.Tensor], dev: int):
+    """Address, row stride and rows of the block table, address and row stride of the positions."""
+    shape, stride = block_table.shape, block_table.stride()
+    if block_table.dtype is not _I32 or block_table.get_device() != dev or len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or stride[1] != 1 or stride[0] < shape[1] and shape[0] > 1:
+        raise _wrong(block_table, "block_table", f"int32 [rows, tokens] on cuda:{dev}")
+    rows, cols = shape
+    bt = (block_table.data_ptr(), stride[0] if rows > 1 else cols, rows)
+    if key_pos is None:
+        return bt, (None, 0)
+    stride = key_pos.stride()
+    if key_pos.dtype is not _I32 or key_pos.get_device() != dev or key_pos.dim() != 2 or key_pos.shape[0] < rows or key_pos.shape[1] < cols or stride[1] != 1 or stride[0] < cols:
+        raise _wrong(key_pos, "key_pos", f"int32, at least [{rows}, {cols}], on cuda:{dev}")
+    return bt, (key_pos.data_ptr(), stride[0])
 
 
-def _weights(mass: torch.Tensor, device, rows: int, Hkv: int, cols: int):
-    p = _is(mass, "mass", _F32, device)
-    if mass.dim() != 3 or mass.shape[0] < rows or mass.shape[1] != Hkv or mass.shape[2] < cols or mass.stride(0) != Hkv * mass.stride(1):
-        raise ValueError(f"mass: at least [{rows}, {Hkv}, {cols}], heads of a row behind one another, expected, got {tuple(mass.shape)} with strides {mass.stride()}")
-    return p, mass.stride(1)
+def _weights(mass: torch.Tensor, dev: int, rows: int, Hkv: int, cols: int):
+    shape, stride = mass.shape, mass.stride()
+    if mass.dtype is not _F32 or mass.get_device() != dev or len(shape) != 3 or shape[0] < rows or shape[1] != Hkv or shape[2] < cols or stride[2] != 1 \
+            or stride[1] < shape[2] or stride[0] != Hkv * stride[1]:
+        raise _wrong(mass, "mass", f"float32, at least [{rows}, {Hkv}, {cols}], the heads of a row behind one another, on cuda:{dev}")
+    return mass.data_ptr(), stride[1]
 
 
-def _shape(device, T, Hq, slopes, bounds, status):
-    return (None if slopes is None else _is(slopes, "slopes", _F32, device, (Hq,)), None if bounds is None else _is(bounds, "bounds", _I32, device, (T, 2)),
-            _is(status, "status", _I32, device))
+def _shape(dev, T, Hq, slopes, bounds, status):
+    return (None if slopes is None else _flat(slopes, "slopes", _F32, dev, (Hq,)), None if bounds is None else _flat(bounds, "bounds", _I32, dev, (T, 2)),
+            _flat(status, "status", _I32, dev, (1,)))
 
 
 def score_bounds(positions: torch.Tensor, *, window: int = 0, doc_first: Optional[torch.Tensor] = None, prefix: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -123,16 +130,14 @@ def attention_shaped_prompt(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     """Rotated queries ``q`` [T, Hq * D] of whole prompts or portions of them -> ``out`` [T, Hq * D] and ``lse`` [T, Hq].  ``runs`` [n, 4] int32 on the
     device: block-table row, tokens held before, index of the first new token in ``q``, new tokens; rows of ``out`` that no run
     names are left alone.  Heads of 64, 128 or 256, at most 128 query heads to a KV head."""
-    L, dev = _library(), _device(q)
+    L, dev, width = _library(), _device(q), Hkv * D
     (qp, ldq), (op, ldo) = _rows(q, "q", dev, T, Hq * D), _rows(out, "out", dev, T, Hq * D)
-    bt, bts = _table(block_table, "block_table", dev, 1, 1)
-    kp, kps = _table(key_pos, "key_pos", dev, block_table.shape[0], block_table.shape[1])
+    (bt, bts, rows), (kp, kps) = _tables(block_table, key_pos, dev)
     sl, bo, st = _shape(dev, T, Hq, slopes, bounds, status)
-    K._check(L.smc_shaped_prompt(qp, ldq, _pool(k_pool, "k_pool", dev, Hkv * D), _pool(v_pool, "v_pool", dev, Hkv * D), min(k_pool.shape[0], v_pool.shape[0]) - 1,
-                                 bt, block_table.shape[1] if block_table.shape[0] == 1 else bts, block_table.shape[0], kp, kps,
-                                 _is(runs, "runs", _I32, dev, (runs.shape[0], 4)), runs.shape[0], op, ldo,
-                                 None if lse is None else _is(lse, "lse", _F32, dev, (T, Hq)), T, Hq, Hkv, D, scale, softcap, sl, bo, st, int(pdl), K._stream()),
-             "smc_shaped_prompt")
+    n = runs.shape[0]
+    K._check(L.smc_shaped_prompt(qp, ldq, _pool(k_pool, "k_pool", dev, width), _pool(v_pool, "v_pool", dev, width), min(k_pool.shape[0], v_pool.shape[0]) - 1, bt, bts, rows,
+                                 kp, kps, _flat(runs, "runs", _I32, dev, (n, 4)), n, op, ldo, None if lse is None else _flat(lse, "lse", _F32, dev, (T, Hq)), T, Hq, Hkv, D,
+                                 scale, softcap, sl, bo, st, pdl, K._stream()), "smc_shaped_prompt")
 
 
 def attention_key_mass(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch.Tensor, runs: torch.Tensor, lse: torch.Tensor, mass: torch.Tensor, *, T: int,
@@ -142,13 +147,12 @@ def attention_key_mass(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch
     (same arguments).  ``runs`` may list fewer tokens than that pass - the last ones of a prompt, say - but a row only once."""
     L, dev = _library(), _device(q)
     qp, ldq = _rows(q, "q", dev, T, Hq * D)
-    bt, bts = _table(block_table, "block_table", dev, 1, 1)
-    kp, kps = _table(key_pos, "key_pos", dev, block_table.shape[0], block_table.shape[1])
+    (bt, bts, rows), (kp, kps) = _tables(block_table, key_pos, dev)
     sl, bo, st = _shape(dev, T, Hq, slopes, bounds, status)
-    mp, ms = _weights(mass, dev, block_table.shape[0], Hkv, block_table.shape[1])
-    K._check(L.smc_shaped_mass(qp, ldq, _pool(k_pool, "k_pool", dev, Hkv * D), k_pool.shape[0] - 1, bt, block_table.shape[1] if block_table.shape[0] == 1 else bts,
-                               block_table.shape[0], kp, kps, _is(runs, "runs", _I32, dev, (runs.shape[0], 4)), runs.shape[0], _is(lse, "lse", _F32, dev, (T, Hq)),
-                               mp, ms, T, Hq, Hkv, D, scale, softcap, sl, bo, st, int(pdl), K._stream()), "smc_shaped_mass")
+    mp, ms = _weights(mass, dev, rows, Hkv, block_table.shape[1])
+    n = runs.shape[0]
+    K._check(L.smc_shaped_mass(qp, ldq, _pool(k_pool, "k_pool", dev, Hkv * D), k_pool.shape[0] - 1, bt, bts, rows, kp, kps, _flat(runs, "runs", _I32, dev, (n, 4)), n,
+                               _flat(lse, "lse", _F32, dev, (T, Hq)), mp, ms, T, Hq, Hkv, D, scale, softcap, sl, bo, st, pdl, K._stream()), "smc_shaped_mass")
 
 
 def shaped_step_work_bytes(bs: int, E: int, Hq: int, Hkv: int, D: int, keys: int = 0) -> int:
@@ -167,17 +171,15 @@ def attention_shaped_step(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     """The last E of the ``lens[s]`` cached tokens of each sequence (``rows``, ``lens`` [bs] int32; a sequence shorter than E is padded in front): queries ``q``
     [bs * E, Hq * D] -> ``out`` and ``lse``.  With ``mass`` (rows listed once) the weights of the step are added to it.  At most 64 rows E * Hq / Hkv, 1024 sequences;
     ``work``: see ``shaped_step_work_bytes``."""
-    L, dev, T = _library(), _device(q), bs * E
+    L, dev, T, width = _library(), _device(q), bs * E, Hkv * D
     (qp, ldq), (op, ldo) = _rows(q, "q", dev, T, Hq * D), _rows(out, "out", dev, T, Hq * D)
-    bt, bts = _table(block_table, "block_table", dev, 1, 1)
-    kp, kps = _table(key_pos, "key_pos", dev, block_table.shape[0], block_table.shape[1])
+    (bt, bts, n), (kp, kps) = _tables(block_table, key_pos, dev)
     sl, bo, st = _shape(dev, T, Hq, slopes, bounds, status)
-    mp, ms = (None, 0) if mass is None else _weights(mass, dev, block_table.shape[0], Hkv, block_table.shape[1])
-    K._check(L.smc_shaped_step(qp, ldq, _pool(k_pool, "k_pool", dev, Hkv * D), _pool(v_pool, "v_pool", dev, Hkv * D), min(k_pool.shape[0], v_pool.shape[0]) - 1, bt,
-                               block_table.shape[1] if block_table.shape[0] == 1 else bts, block_table.shape[0], kp, kps, _is(rows, "rows", _I32, dev, (bs,)),
-                               _is(lens, "lens", _I32, dev, (bs,)), op, ldo, None if lse is None else _is(lse, "lse", _F32, dev, (T, Hq)), mp, ms, bs, E, Hq, Hkv, D,
-                               scale, softcap, sl, bo, _is(work, "work", _U8, dev, work.shape), work.numel(), st, int(pdl), K._stream()),
-             "smc_shaped_step")
+    mp, ms = (None, 0) if mass is None else _weights(mass, dev, n, Hkv, block_table.shape[1])
+    rc = L.smc_shaped_step(qp, ldq, _pool(k_pool, "k_pool", dev, width), _pool(v_pool, "v_pool", dev, width), min(k_pool.shape[0], v_pool.shape[0]) - 1, bt, bts, n, kp, kps,
+                           _flat(rows, "rows", _I32, dev, (bs,)), _flat(lens, "lens", _I32, dev, (bs,)), op, ldo, None if lse is None else _flat(lse, "lse", _F32, dev, (T, Hq)),
+                           mp, ms, bs, E, Hq, Hkv, D, scale, softcap, sl, bo, _flat(work, "work", _U8, dev, (1,)), work.numel(), st, pdl, K._stream())
+    K._check(rc, "smc_shaped_step" if mass is None else "smc_shaped_step with mass")
 
 
 def evict_work_bytes(n_pages: int) -> int:
@@ -194,18 +196,10 @@ def evict_tokens(block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor
     is updated, ``kept`` [n, keep] receives the indices (-1 behind the last).  Weights behind the kept tokens are cleared up to the old length of the row; its other
     entries there are left as they were.  A row may be written by one entry only, and then be read by no other."""
     L, dev = _library(), _device(block_table)
-    R, n = block_table.shape[0], src.shape[0]
-    bt, bts = _table(block_table, "block_table", dev, 1, 1)
-    cols = block_table.shape[1]
-    if bts < cols and R > 1:
-        raise ValueError(f"block_table: rows may not overlap, got strides {block_table.stride()}")
-    kp, kps = _table(key_pos, "key_pos", dev, R, cols)
-    mp, ms = _weights(mass, dev, R, mass.shape[1], cols)
-    pages = refcount.shape[0] - 1
-    if free_stack.shape[0] < pages:
-        raise ValueError(f"free_stack: room for {pages} pages expected, got {free_stack.shape[0]}")
-    K._check(L.smc_evict(bt, bts if R > 1 else cols, kp, kps if R > 1 else max(kps, cols), mp, ms, _is(lens, "lens", _I32, dev, (R,)), R, _is(src, "src", _I32, dev, (n,)),
-                         _is(dst, "dst", _I32, dev, (n,)), n, mass.shape[1], keep, first, last, _is(kept, "kept", _I32, dev, (n, keep)),
-                         _is(refcount, "refcount", _I32, dev, refcount.shape), _is(free_stack, "free_stack", _I32, dev, free_stack.shape),
-                         _is(free_count, "free_count", _I32, dev, free_count.shape), pages, _is(work, "work", _U8, dev, work.shape), work.numel(),
-                         _is(status, "status", _I32, dev), K._stream()), "smc_evict")
+    (bt, bts, R), (kp, kps) = _tables(block_table, key_pos, dev)
+    n, heads, pages = src.shape[0], mass.shape[1], refcount.shape[0] - 1
+    mp, ms = _weights(mass, dev, R, heads, block_table.shape[1])
+    K._check(L.smc_evict(bt, bts, kp, kps, mp, ms, _flat(lens, "lens", _I32, dev, (R,)), R, _flat(src, "src", _I32, dev, (n,)), _flat(dst, "dst", _I32, dev, (n,)), n, heads, keep,
+                         first, last, _flat(kept, "kept", _I32, dev, (n, keep)), _flat(refcount, "refcount", _I32, dev, (pages + 1,)),
+                         _flat(free_stack, "free_stack", _I32, dev, (pages,)), _flat(free_count, "free_count", _I32, dev, (1,)), pages, _flat(work, "work", _U8, dev, (1,)),
+                         work.numel(), _flat(status, "status", _I32, dev, (1,)), K._stream()), "smc_evict")
