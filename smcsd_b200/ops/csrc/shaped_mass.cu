@@ -8,7 +8,9 @@
 //     S_t = K_t Q^T      UMMA 128 x 128 x D, two buffers per key tile in tensor memory
 //     sum                four warps per key tile: exp2(x - lse) of 128 columns, masked by the key's position where a column does not see all keys
 // What bounds it is the exponential, one per (token, head, key) pair; the product is half of the attention's.
-// The grid is persistent: key tiles of all sequences, those with most tokens behind them first.
+// The grid is persistent: key tiles of all sequences, those with most tokens behind them first; the next tile's keys are fetched while one is worked on.  Where sequences bring
+// many tokens the two blocks of a cluster take the steps of a tile by turns and add up their sums through shared memory in their order.
+#include <atomic>
 #include <type_traits>
 
 #include "shaped.cuh"
@@ -17,10 +19,10 @@ namespace smc {
 
 constexpr int MS_LOADERS = 4, MS_Q = 128;
 
-template <int D> struct MsCfg;                        // key tiles of a CTA, slots of the ring of query steps, of them in flight
-template <> struct MsCfg<64> { static constexpr int NT = 2, QU = 6, LAG = 3; };
-template <> struct MsCfg<128> { static constexpr int NT = 2, QU = 4, LAG = 2; };
-template <> struct MsCfg<256> { static constexpr int NT = 1, QU = 2, LAG = 1; };
+template <int D> struct MsCfg;                        // key tiles of a CTA, slots of the ring of query steps, of them in flight, sets of keys in shared memory
+template <> struct MsCfg<64> { static constexpr int NT = 2, QU = 6, LAG = 3, KB = 2; };
+template <> struct MsCfg<128> { static constexpr int NT = 2, QU = 4, LAG = 2, KB = 1; };
+template <> struct MsCfg<256> { static constexpr int NT = 1, QU = 2, LAG = 1, KB = 1; };
 
 struct ShapedMassParams {
   ShapedCache c;
@@ -30,7 +32,7 @@ struct ShapedMassParams {
   const float* lse;              // [T, Hq]
   float* mass;                   // [bt_rows, Hkv, mass_stride]
   long long ld_q, mass_stride;
-  int n_runs, T, Hq, Hkv, pdl;
+  int n_runs, T, Hq, Hkv, pdl, cluster;
   int* status;
 };
 
@@ -43,7 +45,8 @@ struct alignas(16) MsColumns {
 template <int D> struct MsShared {
   static constexpr int SLOTS = MsCfg<D>::QU + 2;      // a step's columns are read until its sums are done, two products behind the ring
   MsColumns col[SLOTS];
-  uint64_t q_full[MsCfg<D>::QU], q_empty[MsCfg<D>::QU], col_full[SLOTS], k_full, s_full[2][2], s_empty[2][2];
+  uint64_t q_full[MsCfg<D>::QU], q_empty[MsCfg<D>::QU], col_full[SLOTS], k_full[2], k_empty[2], s_full[2][2], s_empty[2][2];
+  float sum[MsCfg<D>::NT * 128];                      // of this block, for the cluster
   uint32_t tmem_slot;
   int lo[16], hi[16];
   volatile int abort;
@@ -116,7 +119,7 @@ struct MsTiles {
 
 template <int D, bool CAP, bool BIAS>
 __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shaped_mass_kernel(const ShapedMassParams p) {
-  constexpr int NT = MsCfg<D>::NT, QU = MsCfg<D>::QU, LAG = MsCfg<D>::LAG;
+  constexpr int NT = MsCfg<D>::NT, QU = MsCfg<D>::QU, LAG = MsCfg<D>::LAG, KB = MsCfg<D>::KB;
   constexpr int NPAN = D / 64, PANEL = 128 * 128, TILE = NPAN * PANEL, CPR = D / 8;
   using Shared = MsShared<D>;
   constexpr int SLOTS = Shared::SLOTS;
@@ -124,8 +127,7 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
   __shared__ Shared S;
   const uint32_t raw = smem_u32(ms_smem_raw);
   uint8_t* smem = ms_smem_raw + (((raw + 1023u) & ~1023u) - raw);
-  uint8_t* k_s = smem;                                // [NT] keys
-  uint8_t* q_s = smem + NT * TILE;                    // [QU] query steps
+  uint8_t* q_s = smem + KB * NT * TILE;               // [QU] query steps behind [KB][NT] keys
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr int LOAD_WARP = 4 * NT, MMA_WARP = LOAD_WARP + MS_LOADERS;
   const int G = p.Hq / p.Hkv, TT = 128 / G;           // tokens of a step
@@ -139,7 +141,10 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
       mbar_init(&S.q_empty[i], NT);
     }
     for (int i = 0; i < SLOTS; ++i) mbar_init(&S.col_full[i], MS_LOADERS);
-    mbar_init(&S.k_full, MS_LOADERS);
+    for (int i = 0; i < KB; ++i) {
+      mbar_init(&S.k_full[i], MS_LOADERS);
+      mbar_init(&S.k_empty[i], NT);
+    }
     for (int t = 0; t < NT; ++t)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&S.s_full[t][i], 1);
@@ -158,9 +163,10 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
   const long long items = all.count(1) * p.Hkv;
   bool dead = false;                                  // a wait of this warp ran out: it goes on to the end without work
   uint32_t u0 = 0, k_use = 0;                         // steps and key tiles so far: barriers run on from item to item
-  for (long long base = 0, round = 0; base < items; base += gridDim.x, ++round) {
+  const int C = p.cluster, rank = C > 1 ? (int)cluster_ctarank() : 0, groups = gridDim.x / C, group = blockIdx.x / C;
+  for (long long base = 0, round = 0; base < items; base += groups, ++round) {
     // every second round runs backwards, so that who had a long tile gets a short one
-    const long long item = base + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    const long long item = base + (round & 1 ? groups - 1 - group : group);
     ShapedRun run{0, 0, 0, 0};
     int number = 0, tile = 0;
     bool have = item < items && all.find(item / p.Hkv, run, number, tile);
@@ -195,16 +201,17 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
       tb = 0;
       for (int w = 0; w < (int)(blockDim.x >> 5); ++w) { ta = min(ta, S.lo[w]); tb = max(tb, S.hi[w]); }
     }
-    const int n_steps = tb > ta ? (tb - ta + TT - 1) / TT : 0;
-    if (n_steps == 0 || dead) continue;
-
-    if (warp >= LOAD_WARP && warp < MMA_WARP) {
+    const int all_steps = tb > ta ? (tb - ta + TT - 1) / TT : 0, n_steps = (all_steps - rank + C - 1) / C;     // this block's: rank, rank + C, ...
+    uint8_t* k_s = smem + (k_use % KB) * NT * TILE;
+    float total = 0.f;
+    if (n_steps <= 0 || dead) {
+    } else if (warp >= LOAD_WARP && warp < MMA_WARP) {
       // ================================================================= loaders
       const int lw = warp - LOAD_WARP;
-      bool go = u0 == 0 || ms_wait(S, p.status, &S.q_empty[(u0 - 1) % QU], ((u0 - 1) / QU) & 1u);      // products with the keys before are done
+      bool go = k_use < KB || ms_wait(S, p.status, &S.k_empty[k_use % KB], (k_use / KB - 1) & 1u);     // products with the keys before are done
       go = __all_sync(0xffffffffu, go);
-      if (!go) { dead = true; continue; }
-      {                                               // keys: this warp's 32 of each tile
+      dead = !go;
+      if (go) {                                       // keys: this warp's 32 of each tile
         const int* bt = p.c.block_table + (size_t)run.row * p.c.bt_stride;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -222,25 +229,33 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       }
-      for (int j = 0; j < n_steps; ++j) {
-        const uint32_t u = u0 + j, st = u % QU;
-        // this lane's column
-        const int cl = lw * 32 + lane, tok = ta + j * TT + cl / G, h = hbase + cl % G;
-        const bool live = cl < TT * G && tok < tb;
-        float nl = -INFINITY, posf = 0.f, first = 0.f, last = (float)SH_POS_END, slope = 0.f;
-        if (live) {
-          const float lse = p.lse[(size_t)(run.at + tok) * p.Hq + h];
-          const int pos = pos_of(run.held + tok);
-          int2 b = shaped_bounds(p.c, run.at + tok, pos);
-          if (lse == -INFINITY) b = make_int2(SH_POS_END, -1);        // it has seen nothing
-          else nl = -lse * SH_LOG2E;
-          posf = (float)pos;
-          first = (float)b.x;
-          last = (float)b.y;
-          if (BIAS) slope = -p.c.slopes[h] * SH_LOG2E;
+      // this lane's column of a step, read one step ahead
+      const int cl = lw * 32 + lane, ct = cl / G, h = hbase + cl % G;
+      const int row_off = ct * (int)p.ld_q + cl % G * D;               // of its query row, from the step's first token on (tokens of a step: at most 128)
+      struct Column { float lse; int pos; int2 see; bool live; } next;
+      const float slope = BIAS && cl < TT * G ? -p.c.slopes[h] * SH_LOG2E : 0.f;
+      auto column = [&](int j) {
+        const int tok = ta + (rank + j * C) * TT + ct;
+        Column c{-INFINITY, 0, make_int2(0, SH_POS_END), cl < TT * G && tok < tb && j < n_steps};
+        if (c.live) {
+          c.lse = p.lse[(size_t)(run.at + tok) * p.Hq + h];
+          c.pos = pos_of(run.held + tok);
+          c.see = shaped_bounds(p.c, run.at + tok, c.pos);
         }
+        return c;
+      };
+      if (go) next = column(0);
+      for (int j = 0; go && j < n_steps; ++j) {
+        const uint32_t u = u0 + j, st = u % QU;
+        const int step0 = ta + (rank + j * C) * TT;
+        const Column mine = next;
+        next = column(j + 1);
+        const bool live = mine.live, seen = mine.lse != -INFINITY;
+        const float nl = seen ? -mine.lse * SH_LOG2E : -INFINITY, posf = (float)mine.pos;
+        // a token that has seen nothing sees no key
+        const float first = !live || seen ? (float)mine.see.x : (float)SH_POS_END, last = !live || seen ? (float)mine.see.y : -1.f;
         const bool ok = u < QU || ms_wait(S, p.status, &S.q_empty[st], (u / QU - 1) & 1u);
-        if (!__all_sync(0xffffffffu, ok)) { go = false; break; }
+        if (!__all_sync(0xffffffffu, ok)) { go = false; dead = true; break; }
         MsColumns& col = S.col[u % SLOTS];
         col.neg_lse[cl] = nl;
         col.pos[cl] = posf;
@@ -252,29 +267,29 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         if (lane == 0) { col.max_first[lw] = mf; col.min_last[lw] = ml; col.min_pos4[lw] = mp; }
         __syncwarp();
         if (lane == 0) mbar_arrive(&S.col_full[u % SLOTS]);
-        const uint32_t dst0 = smem_u32(q_s + (size_t)st * TILE);
-#pragma unroll 4
-        for (int idx = lane; idx < 32 * CPR; idx += 32) {
-          const int rl = idx / CPR, c = idx % CPR, r = lw * 32 + rl, tk = ta + j * TT + r / G;
-          const bool real = r < TT * G && tk < tb;
-          const __nv_bfloat16* src = p.q + (size_t)(run.at + (real ? tk : ta)) * p.ld_q + (size_t)(hbase + r % G) * D + c * 8;
-          const uint32_t dst = dst0 + (uint32_t)((c >> 3) * PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+        // the row of every lane's column, 16 bytes a lane: chunk lane % CPR of the rows lane / CPR, + 32 / CPR, ...
+        const __nv_bfloat16* q0 = p.q + (size_t)(run.at + step0) * p.ld_q + (size_t)hbase * D + lane % CPR * 8;
+        const uint32_t dst0 = smem_u32(q_s + (size_t)st * TILE) + (uint32_t)((lane % CPR >> 3) * PANEL);
+#pragma unroll
+        for (int r0 = 0; r0 < 32; r0 += 32 / CPR) {
+          const int rl = r0 + lane / CPR, r = lw * 32 + rl;
+          const int off = __shfl_sync(0xffffffffu, live ? row_off : -1, rl);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                       ::"r"(dst0 + (uint32_t)(r * 128 + (((lane % CPR & 7) ^ (r & 7)) << 4))), "l"(q0 + max(off, 0)), "r"(off >= 0 ? 16 : 0) : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
         if (j >= LAG - 1) {                           // the keys, then step j - LAG, have landed: hand them over
           asm volatile("cp.async.wait_group %0;" ::"n"(LAG) : "memory");
           fence_proxy_async();
           __syncwarp();
-          if (lane == 0) mbar_arrive(j == LAG - 1 ? &S.k_full : &S.q_full[(u - LAG) % QU]);
+          if (lane == 0) mbar_arrive(j == LAG - 1 ? &S.k_full[k_use % KB] : &S.q_full[(u - LAG) % QU]);
         }
       }
       asm volatile("cp.async.wait_group 0;" ::: "memory");
       fence_proxy_async();
       __syncwarp();
-      if (!go) { dead = true; continue; }
-      if (lane == 0) {
-        if (n_steps < LAG) mbar_arrive(&S.k_full);
+      if (go && lane == 0) {
+        if (n_steps < LAG) mbar_arrive(&S.k_full[k_use % KB]);
         for (int j = max(0, n_steps - LAG); j < n_steps; ++j) mbar_arrive(&S.q_full[(u0 + j) % QU]);
       }
     } else if (warp >= MMA_WARP) {
@@ -284,7 +299,7 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
       if (elect_one()) {
         constexpr uint32_t idesc = umma_idesc_bf16(128, MS_Q);
         const uint32_t k_addr = smem_u32(k_s) + t * TILE;
-        ok = ms_wait(S, p.status, &S.k_full, k_use & 1u);
+        ok = ms_wait(S, p.status, &S.k_full[k_use % KB], (k_use / KB) & 1u);
         for (int j = 0; ok && j < n_steps; ++j) {
           const uint32_t u = u0 + j, st = u % QU, buf = u & 1u;
           ok = ms_wait(S, p.status, &S.q_full[st], (u / QU) & 1u) && (u < 2 || ms_wait(S, p.status, &S.s_empty[t][buf], (u / 2 - 1) & 1u));
@@ -299,9 +314,10 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
                            umma_desc_k_sw128(q_addr + pan * PANEL) + 2 * k, idesc, (pan | k) ? 1u : 0u);
           umma_commit(&S.s_full[t][buf]);
           umma_commit(&S.q_empty[st]);
+          if (j == n_steps - 1) umma_commit(&S.k_empty[k_use % KB]);
         }
       }
-      if (!__all_sync(0xffffffffu, ok)) { dead = true; continue; }
+      dead = !__all_sync(0xffffffffu, ok);
     } else {
       // ================================================================= sums (one key per thread)
       const int t = warp >> 2, r = (warp & 3) * 32 + lane, k = k0 + t * 128 + r;
@@ -310,13 +326,11 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
       const float mul = p.c.mul, cap_in = p.c.cap_in, cap_out = p.c.cap_out;
       const uint64_t mul2 = f2_pair(mul, mul), kpos2 = f2_pair(kpos, kpos);
       const ShapedCapNear<4> near(cap_in, cap_out, mul);
-      float total = 0.f;
-      bool alive = true;
       for (int j = 0; j < n_steps; ++j) {
         const uint32_t u = u0 + j, buf = u & 1u;
         const MsColumns& col = S.col[u % SLOTS];
         if (!__all_sync(0xffffffffu, ms_wait(S, p.status, &S.s_full[t][buf], (u / 2) & 1u) &&
-                                         ms_wait(S, p.status, &S.col_full[u % SLOTS], (u / SLOTS) & 1u))) { alive = false; break; }
+                                         ms_wait(S, p.status, &S.col_full[u % SLOTS], (u / SLOTS) & 1u))) { dead = true; break; }
         tc_fence_after();
         const float4 mf = *reinterpret_cast<const float4*>(col.max_first), ml = *reinterpret_cast<const float4*>(col.min_last);
         const bool full = __all_sync(0xffffffffu, kpos >= fmaxf(fmaxf(mf.x, mf.y), fmaxf(mf.z, mf.w)) && kpos <= fminf(fminf(ml.x, ml.y), fminf(ml.z, ml.w)));
@@ -386,9 +400,20 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         const float2 a = f2_unpair(part[0]), b = f2_unpair(part[1]);
         total += (a.x + a.y) + (b.x + b.y);
       }
-      if (!alive) { dead = true; continue; }
-      if (k < keys) p.mass[((size_t)run.row * p.Hkv + kvh) * p.mass_stride + k] += total;
+      if (C == 1 && !dead && k < keys) p.mass[((size_t)run.row * p.Hkv + kvh) * p.mass_stride + k] += total;
     }
+    if (C > 1 && all_steps > 0) {                     // the blocks' sums in their order, a part of the keys by each block
+      if (warp < LOAD_WARP) S.sum[threadIdx.x] = dead ? 0.f : total;
+      cluster_sync();
+      const int share = NT * 128 / C, i = rank * share + threadIdx.x;
+      if (threadIdx.x < share && k0 + i < keys) {
+        float all_of = 0.f;
+        for (int c = 0; c < C; ++c) all_of += ld_dsmem_f32(smem_u32(&S.sum[i]), c);
+        p.mass[((size_t)run.row * p.Hkv + kvh) * p.mass_stride + k0 + i] += all_of;
+      }
+      cluster_sync();
+    }
+    if (n_steps <= 0) continue;
     u0 += n_steps;
     ++k_use;
   }
@@ -399,19 +424,34 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
 
 template <int D, bool CAP, bool BIAS>
 static int launch_shaped_mass(const ShapedMassParams& p, cudaStream_t st) {
-  constexpr size_t smem = (size_t)(MsCfg<D>::NT + MsCfg<D>::QU) * D * 256 + 1024;
+  constexpr size_t smem = (size_t)(MsCfg<D>::KB * MsCfg<D>::NT + MsCfg<D>::QU) * D * 256 + 1024;
   static_assert(smem + sizeof(MsShared<D>) <= 232448, "shared memory");
   CUDA_CHECK_RET(cudaFuncSetAttribute(shaped_mass_kernel<D, CAP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(148);
   cfg.blockDim = dim3((5 * MsCfg<D>::NT + MS_LOADERS) * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = p.pdl ? 1 : 0;
+  // as many clusters as the device holds at once (fewer than its SMs would make: a cluster stays inside a GPC), looked up once for each device
+  static std::atomic<int> held[64][9];
+  int dev = 0;
+  CUDA_CHECK_RET(cudaGetDevice(&dev));
+  int clusters = dev < 64 ? held[dev][p.cluster].load(std::memory_order_relaxed) : 0;
+  if (clusters == 0) {
+    cfg.gridDim = dim3((unsigned)p.cluster);
+    cfg.numAttrs = 1;
+    CUDA_CHECK_RET(cudaOccupancyMaxActiveClusters(&clusters, shaped_mass_kernel<D, CAP, BIAS>, &cfg));
+    if (clusters < 1) return -164;
+    if (dev < 64) held[dev][p.cluster].store(clusters, std::memory_order_relaxed);
+  }
+  cfg.gridDim = dim3((unsigned)(clusters * p.cluster));
+  cfg.numAttrs = p.pdl ? 2 : 1;
   CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, shaped_mass_kernel<D, CAP, BIAS>, p));
   return 0;
 }
@@ -426,7 +466,7 @@ SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, i
   using namespace smc;
   if (n_runs <= 0 || T <= 0) return 0;
   if (Hkv < 1 || Hq < Hkv || Hq % Hkv || Hq / Hkv > 128 || (D != 64 && D != 128 && D != 256)) return -160;
-  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(runs)) & 15 || (ld_q & 7) ||
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(runs)) & 15 || (ld_q & 7) || ld_q > (1 << 23) ||
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -161;
   if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -162;
@@ -435,6 +475,10 @@ SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, i
   p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.runs = (const int4*)runs; p.lse = lse; p.mass = mass;
   p.ld_q = ld_q; p.mass_stride = mass_stride; p.n_runs = n_runs; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.pdl = pdl; p.status = status;
+  // Two blocks to a key tile where sequences bring 16 steps and more: the first tile of a sequence, which all its tokens see, is half as long then.  4096 tokens, 32 heads of
+  // 128 on 8: one block 318 us, two 200, four 240, eight 297 - a tile costs 8 us before its first sum in every block.
+  const long long steps = (long long)T / n_runs * (Hq / Hkv) / 128;
+  p.cluster = steps >= 16 ? 2 : 1;
 #define SMC_SHAPED_MASS(DD)                                                                                            \
   if (D == DD) {                                                                                                       \
     if (cap > 0.f) return slopes ? launch_shaped_mass<DD, true, true>(p, st) : launch_shaped_mass<DD, true, false>(p, st); \
