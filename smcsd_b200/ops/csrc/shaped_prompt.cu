@@ -456,25 +456,28 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
           top += slope * (slope > 0.f ? fmaxf(a, b) : fminf(a, b));
         }
       } else {
-        const bool within = CAP && __all_sync(0xffffffffu, reach <= SH_TANH5_REACH);
+        // (the few scores beyond reach in a loop of their own: between the others their code would lie 64 times in the way, 10 us of a first step)
         const ShapedCapNear<5> by_five(cap_in, cap_out, mul);
+        if (CAP && __any_sync(0xffffffffu, !(reach <= SH_TANH5_REACH))) {
+#pragma unroll
+          for (int i = 0; i < BK; ++i) x[i] = __float_as_uint(shaped_cap(val(i), cap_in, cap_out));
+        } else {
+#pragma unroll
+          for (int i = 0; i < BK; i += 2) {
+            const float2 v = f2_unpair(CAP ? by_five(pair(i), 0ull) : f2_mul(pair(i), f2_pair(mul, mul)));
+            x[i] = __float_as_uint(v.x);
+            x[i + 1] = __float_as_uint(v.y);
+          }
+        }
         top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < BK; i += 2) {
-          float2 v;
-          if (!CAP) v = f2_unpair(f2_mul(pair(i), f2_pair(mul, mul)));
-          else if (within) v = f2_unpair(by_five(pair(i), 0ull));
-          else v = make_float2(shaped_cap(val(i), cap_in, cap_out), shaped_cap(val(i + 1), cap_in, cap_out));
-          const float at0 = pos0 + pos[i], at1 = pos0 + pos[i + 1];
-          if (BIAS) {
-            v.x = fmaf(fabsf(at0 - pos_row), slope, v.x);
-            v.y = fmaf(fabsf(at1 - pos_row), slope, v.y);
-          }
-          if (!(at0 >= first_seen && at0 <= last_seen)) v.x = -INFINITY;               // probability zero
-          if (!(at1 >= first_seen && at1 <= last_seen)) v.y = -INFINITY;
-          x[i] = __float_as_uint(v.x);
-          x[i + 1] = __float_as_uint(v.y);
-          top = shaped_max3(top, v.x, v.y);
+        for (int i = 0; i < BK; ++i) {
+          const float at = pos0 + pos[i];
+          float v = val(i);
+          if (BIAS) v = fmaf(fabsf(at - pos_row), slope, v);
+          v = at >= first_seen && at <= last_seen ? v : -INFINITY;    // probability zero
+          x[i] = __float_as_uint(v);
+          top = fmaxf(top, v);
         }
       }
       const bool grow = top > m_ref + 8.f;            // also true for the first visible key (m_ref = -inf)
