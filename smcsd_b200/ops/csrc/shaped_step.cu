@@ -358,6 +358,10 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
       }
     }
     named_bar(1, THREADS);                                           // rows are known
+    // keys between these are seen by all of this warp's rows
+    const int my_row = mt * NQ * 8 + lane;
+    const bool has_row = lane < NQ * 8 && my_row < M;
+    const float seen_from = warp_max(has_row ? row_s[my_row].x : -1.f), seen_to = -warp_max(has_row ? -row_s[my_row].y : -(float)SH_POS_END);
     float m[NQ][2], l[NQ][2], o[NQ][D / 16][4];                      // of columns 2 c4, 2 c4 + 1
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
@@ -400,10 +404,19 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
           const int pos = p.c.key_pos != nullptr ? pos_s[st * KT + k0 + g + 8 * h] : key.begin + i0 + 8 * h;
           kp[h] = i0 + 8 * h < key.n ? (float)pos : -1.f;
         }
+        const bool plain = p.c.slopes == nullptr && __all_sync(0xffffffffu, kp[0] >= seen_from && kp[1] >= 0.f && kp[1] <= seen_to);
         uint32_t pb[NQ][2];
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
           float top[2] = {m[q][0], m[q][1]};
+          if (plain) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float v = sc[q][i] + sd[q][i];
+              sc[q][i] = cap_in > 0.f ? shaped_cap(v, cap_in, cap_out) : v * mul;
+              top[i & 1] = fmaxf(top[i & 1], sc[q][i]);
+            }
+          } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float4 row = row_s[(mt * NQ + q) * 8 + 2 * c4 + (i & 1)];
@@ -413,6 +426,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
             v = kp[i >> 1] >= row.x && kp[i >> 1] <= row.y ? v : -INFINITY;
             sc[q][i] = v;
             top[i & 1] = fmaxf(top[i & 1], v);
+          }
           }
           if (p.scores != nullptr && x < p.score_tiles) {
             const int r = (mt * NQ + q) * 8 + 2 * c4;
