@@ -85,8 +85,8 @@ __device__ __forceinline__ int step_first(int w, int workers, int total) { retur
 // the worker that has tile x
 __device__ __forceinline__ int step_owner(int x, int workers, int total) { return (int)((((long long)x + 1) * workers - 1) / total); }
 
-__device__ __forceinline__ void st_cp16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+__device__ __forceinline__ void st_cp16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
 }
 __device__ __forceinline__ void st_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
     // ================================================================= loaders: KW keys of each tile a warp
     const int lw = warp - Cfg::WARPS, kl0 = lw * KW + lane % KW;
     const long long row_bytes = (long long)p.Hkv * D * 2;
+    const uint64_t policy = l2_policy_evict_first();                 // read once: L2 is for the scores
     // what this lane copies: with BULK a row of K or V, else chunk lane % CPR of the rows lane / CPR, + 32 / CPR, ...
     const int c = Cfg::BULK ? 0 : lane % CPR, r0 = Cfg::BULK ? lane & 15 : lane / CPR;
     const char* from_k = reinterpret_cast<const char*>((Cfg::BULK && lane >= 16 ? p.v_pool : p.k_pool) + (size_t)kvh * D + c * 8);
@@ -299,14 +300,14 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
           __syncwarp();
           if (lane == 0) mbar_expect_tx(&S.full[st], 32 * D * 2);
           __syncwarp();
-          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                       ::"r"(to), "l"(from_k + pg * row_bytes), "r"(D * 2), "r"(smem_u32(&S.full[st])) : "memory");
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+                       ::"r"(to), "l"(from_k + pg * row_bytes), "r"(D * 2), "r"(smem_u32(&S.full[st])), "l"(policy) : "memory");
         } else {
 #pragma unroll
           for (int r = 0; r < KW; r += 32 / CPR) {
             const long long off = __shfl_sync(0xffffffffu, pg, r0 + r) * row_bytes;
-            st_cp16(to + (uint32_t)(r * LD * 2), from_k + off);
-            st_cp16(to + (uint32_t)(r * LD * 2) + (uint32_t)Cfg::KV, from_v + off);
+            st_cp16(to + (uint32_t)(r * LD * 2), from_k + off, policy);
+            st_cp16(to + (uint32_t)(r * LD * 2) + (uint32_t)Cfg::KV, from_v + off, policy);
           }
           __syncwarp();                                              // each lane arrives once its own copies have landed
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&S.full[st])) : "memory");
