@@ -39,6 +39,7 @@ struct ShapedMassParams {
 // What a step's query rows bring along, by column
 struct alignas(16) MsColumns {
   float neg_lse[MS_Q], pos[MS_Q], first[MS_Q], last[MS_Q], slope[MS_Q];
+  float reach[MS_Q];                                  // neg_lse and slope times the distance from the tile's first key: what a key in front of the token adds is linear
   float max_first[4], min_last[4], min_pos4[4];       // over 32 columns each: a key between the first two is seen by every column
 };
 
@@ -68,29 +69,29 @@ __device__ __forceinline__ bool ms_wait(Shared& S, int* status, uint64_t* bar, u
   }
 }
 
-// All tiles of `kt` keys of all sequences, those with most tokens behind their first key in front; used by whole warps.
+// All tiles of KT keys of all sequences, those with most tokens behind their first key in front; used by whole warps.
+template <int KT>
 struct MsTiles {
   const ShapedMassParams& p;
-  int kt;
   ShapedRun mine;
-  __device__ MsTiles(const ShapedMassParams& params, int keys) : p(params), kt(keys) { mine = run_of((int)threadIdx.x & 31); }
+  __device__ explicit MsTiles(const ShapedMassParams& params) : p(params) { mine = run_of((int)threadIdx.x & 31); }
   __device__ ShapedRun run_of(int s) const { return s < p.n_runs ? shaped_run(p.c, p.runs, s, p.T, p.status) : ShapedRun{0, 0, 0, 0}; }
   // tiles of run r with at least `tokens` of its new tokens at or behind their first key: the first ones of the row
-  __device__ int of_run(const ShapedRun& r, int tokens) const { return tokens > r.n ? 0 : (r.held + r.n - tokens) / kt + 1; }
-  __device__ long long count(int tokens) const {
+  __device__ int of_run(const ShapedRun& r, int tokens) const { return tokens > r.n ? 0 : (int)((unsigned)(r.held + r.n - tokens) / KT) + 1; }
+  __device__ int count(int tokens) const {
     int n = of_run(mine, tokens);
     for (int s = (threadIdx.x & 31) + 32; s < p.n_runs; s += 32) n += of_run(run_of(s), tokens);
-    return (long long)__reduce_add_sync(0xffffffffu, (unsigned)n);
+    return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
   }
   // tile number `want`: its run, the run's number and the tile inside it
-  __device__ bool find(long long want, ShapedRun& run, int& number, int& tile) const {
+  __device__ bool find(int want, ShapedRun& run, int& number, int& tile) const {
     const int lane = threadIdx.x & 31;
     int lo = 1, hi = p.T + 1;                         // count(lo) > want >= count(hi)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (count(mid) > want) lo = mid; else hi = mid;
     }
-    int left = (int)(want - count(lo + 1));
+    int left = want - count(lo + 1);
     for (int s0 = 0; s0 < p.n_runs; s0 += 32) {
       const ShapedRun r = s0 == 0 ? mine : run_of(s0 + lane);
       const int more = of_run(r, lo + 1), n = of_run(r, lo) - more;
@@ -159,14 +160,14 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
   const uint32_t tmem_base = S.tmem_slot;
   if (p.pdl) { pdl_launch_dependents(); pdl_wait_prior_grid(); }
 
-  const MsTiles all(p, NT * 128);
-  const long long items = all.count(1) * p.Hkv;
+  const MsTiles<NT * 128> all(p);
+  const int items = all.count(1) * p.Hkv;             // (at most the table's entries over 128, times the heads)
   bool dead = false;                                  // a wait of this warp ran out: it goes on to the end without work
   uint32_t u0 = 0, k_use = 0;                         // steps and key tiles so far: barriers run on from item to item
   const int C = p.cluster, rank = C > 1 ? (int)cluster_ctarank() : 0, groups = gridDim.x / C, group = blockIdx.x / C;
-  for (long long base = 0, round = 0; base < items; base += groups, ++round) {
+  for (int base = 0, round = 0; base < items; base += groups, ++round) {
     // every second round runs backwards, so that who had a long tile gets a short one
-    const long long item = base + (round & 1 ? groups - 1 - group : group);
+    const int item = base + (round & 1 ? groups - 1 - group : group);
     ShapedRun run{0, 0, 0, 0};
     int number = 0, tile = 0;
     bool have = item < items && all.find(item / p.Hkv, run, number, tile);
@@ -178,9 +179,10 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         have = false;
       }
     }
-    const int kvh = (int)(item % p.Hkv), hbase = kvh * G, keys = run.held + run.n, k0 = tile * NT * 128;
+    const int kvh = item % p.Hkv, hbase = kvh * G, keys = run.held + run.n, k0 = tile * NT * 128;
     const int* kp = p.c.key_pos != nullptr ? p.c.key_pos + (size_t)run.row * p.c.kp_stride : nullptr;
     auto pos_of = [&](int idx) { return kp != nullptr ? kp[idx] : idx; };
+    const float base_pos = BIAS && have ? (float)pos_of(k0) : 0.f;
     // new tokens [ta, tb) of the run that may see one of the keys
     int ta = max(0, k0 - run.held), tb = have ? run.n : 0;
     if (p.c.bounds != nullptr) {
@@ -261,7 +263,10 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         col.pos[cl] = posf;
         col.first[cl] = first;
         col.last[cl] = last;
-        if (BIAS) col.slope[cl] = slope;
+        if (BIAS) {
+          col.slope[cl] = slope;
+          col.reach[cl] = nl + slope * (posf - base_pos);
+        }
         const float mf = warp_max(first), ml = -warp_max(-last);
         const float mp = BIAS ? -warp_max(live ? -posf : -(float)SH_POS_END) : 0.f;
         if (lane == 0) { col.max_first[lw] = mf; col.min_last[lw] = ml; col.min_pos4[lw] = mp; }
@@ -324,8 +329,10 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
       const uint32_t ts = tmem_base + (uint32_t)t * 256u + (((uint32_t)((warp & 3) * 32)) << 16);
       const float kpos = k < keys ? (float)pos_of(k) : -1.f;
       const float mul = p.c.mul, cap_in = p.c.cap_in, cap_out = p.c.cap_out;
-      const uint64_t mul2 = f2_pair(mul, mul), kpos2 = f2_pair(kpos, kpos);
+      const uint64_t mul2 = f2_pair(mul, mul), kpos2 = f2_pair(kpos, kpos), from_base2 = f2_pair(base_pos - kpos, base_pos - kpos);
       const ShapedCapNear<4> near(cap_in, cap_out, mul);
+      float* to = p.mass + ((size_t)run.row * p.Hkv + kvh) * p.mass_stride + k;
+      const float before = C == 1 && k < keys ? *to : 0.f;          // long back when the sum is there
       for (int j = 0; j < n_steps; ++j) {
         const uint32_t u = u0 + j, buf = u & 1u;
         const MsColumns& col = S.col[u % SLOTS];
@@ -336,23 +343,26 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         const bool full = __all_sync(0xffffffffu, kpos >= fmaxf(fmaxf(mf.x, mf.y), fmaxf(mf.z, mf.w)) && kpos <= fminf(fminf(ml.x, ml.y), fminf(ml.z, ml.w)));
         const float4 mp = *reinterpret_cast<const float4*>(col.min_pos4);
         uint64_t part[2] = {0ull, 0ull};              // a step's sum in four parts ahead of the running one: short chains of additions
-        const bool cause = !BIAS || __all_sync(0xffffffffu, kpos <= fminf(fminf(mp.x, mp.y), fminf(mp.z, mp.w)));     // every column lies behind this key
-        // exp2 of what `shaped` makes of pairs of scores and negated references
-        auto add_up = [&](const uint32_t (&w)[32], int c0, auto masked, auto shaped) {
+        const bool behind = !BIAS || __all_sync(0xffffffffu, kpos <= fminf(fminf(mp.x, mp.y), fminf(mp.z, mp.w)));    // every column lies behind this key
+        // exp2 of what `shaped` makes of pairs of scores and what is added to them; `plain`: every key is in front of every token and seen by it
+        auto add_up = [&](const uint32_t (&w)[32], int c0, auto plain, auto shaped) {
+          constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(&col.neg_lse[c0 + i]);
+            const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(BIAS && PLAIN ? &col.reach[c0 + i] : &col.neg_lse[c0 + i]);
             uint64_t off[2] = {nl.x, nl.y};
             if (BIAS) {
-              const ulonglong2 at = *reinterpret_cast<const ulonglong2*>(&col.pos[c0 + i]), sl = *reinterpret_cast<const ulonglong2*>(&col.slope[c0 + i]);
+              const ulonglong2 sl = *reinterpret_cast<const ulonglong2*>(&col.slope[c0 + i]);
+              if constexpr (PLAIN) {
+                off[0] = f2_fma(from_base2, sl.x, off[0]);
+                off[1] = f2_fma(from_base2, sl.y, off[1]);
+              } else {
+                const ulonglong2 at = *reinterpret_cast<const ulonglong2*>(&col.pos[c0 + i]);
 #pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                uint64_t d = f2_fma(kpos2, f2_pair(-1.f, -1.f), k ? at.y : at.x);     // column less key
-                if (!cause) {
-                  const float2 v = f2_unpair(d);
-                  d = f2_pair(fabsf(v.x), fabsf(v.y));
+                for (int k = 0; k < 2; ++k) {
+                  const float2 v = f2_unpair(f2_fma(kpos2, f2_pair(-1.f, -1.f), k ? at.y : at.x));
+                  off[k] = f2_fma(f2_pair(fabsf(v.x), fabsf(v.y)), k ? sl.y : sl.x, off[k]);
                 }
-                off[k] = f2_fma(d, k ? sl.y : sl.x, off[k]);
               }
             }
 #pragma unroll
@@ -360,7 +370,7 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
               const int c = c0 + i + 2 * k;
               const float2 v = f2_unpair(shaped(f2_pair(__uint_as_float(w[i + 2 * k]), __uint_as_float(w[i + 2 * k + 1])), off[k]));
               float e0 = shaped_ex2(v.x), e1 = shaped_ex2(v.y);
-              if constexpr (decltype(masked)::value) {
+              if constexpr (!PLAIN) {
                 e0 = kpos >= col.first[c] && kpos <= col.last[c] ? e0 : 0.f;
                 e1 = kpos >= col.first[c + 1] && kpos <= col.last[c + 1] ? e1 : 0.f;
               }
@@ -385,13 +395,13 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
             for (int i = 0; i < 64; i += 2) far = shaped_max3(far, fabsf(__uint_as_float(w[i >> 5][i & 31])), fabsf(__uint_as_float(w[i >> 5][(i & 31) + 1])));
             reach = __all_sync(0xffffffffu, far * cap_in <= near.reach);
           }
-          if (full && reach) {
+          if (full && reach && behind) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-              add_up(w[h], c0 + 32 * h, std::false_type(), [&](uint64_t x, uint64_t off) { return CAP ? near(x, off) : f2_fma(x, mul2, off); });
+              add_up(w[h], c0 + 32 * h, std::true_type(), [&](uint64_t x, uint64_t off) { return CAP ? near(x, off) : f2_fma(x, mul2, off); });
           } else {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) add_up(w[h], c0 + 32 * h, std::true_type(), number_by_number);
+            for (int h = 0; h < 2; ++h) add_up(w[h], c0 + 32 * h, std::false_type(), number_by_number);
           }
         }
         tc_fence_before();
@@ -400,7 +410,7 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         const float2 a = f2_unpair(part[0]), b = f2_unpair(part[1]);
         total += (a.x + a.y) + (b.x + b.y);
       }
-      if (C == 1 && !dead && k < keys) p.mass[((size_t)run.row * p.Hkv + kvh) * p.mass_stride + k] += total;
+      if (C == 1 && !dead && k < keys) *to = before + total;
     }
     if (C > 1 && all_steps > 0) {                     // the blocks' sums in their order, a part of the keys by each block
       if (warp < LOAD_WARP) S.sum[threadIdx.x] = dead ? 0.f : total;
