@@ -412,7 +412,7 @@ def test_prompt_mass_eviction_and_steps_together():
     q, q1 = torch.randn(n, Hq * D, device=DEV).bfloat16(), torch.randn(2, Hq * D, device=DEV).bfloat16()
     new_k, new_v = (torch.randn(2, Hkv * D, device=DEV).bfloat16() for _ in range(2))
     out, lse, out1 = torch.zeros_like(q), torch.zeros(n, Hq, device=DEV), torch.zeros_like(q1)
-    kept, kept2 = torch.zeros(1, keep, dtype=torch.int32, device=DEV), torch.zeros(2, 100, dtype=torch.int32, device=DEV)
+    kept, whole, kept2 = (torch.zeros(*x, dtype=torch.int32, device=DEV) for x in ((1, keep), (1, keep), (2, 100)))
     ework = torch.zeros(N.evict_work_bytes(a.size), dtype=torch.uint8, device=DEV)
     swork = torch.zeros(N.shaped_step_work_bytes(2, 1, Hq, Hkv, D, 2 * (keep + 1)), dtype=torch.uint8, device=DEV)
     one, two, both = (torch.tensor(x, device=DEV).int() for x in ([1], [2], [1, 2]))
@@ -427,7 +427,7 @@ def test_prompt_mass_eviction_and_steps_together():
         N.attention_key_mass(q, c.k, table, runs, lse, mass, T=n, **shape)
         pool = (a.refcount, a.free_stack, a.free_count)
         N.evict_tokens(table, one, one, ln, mass, *pool, keep=keep, first=4, last=30, key_pos=pos, kept=kept, work=ework, status=st)
-        N.evict_tokens(table, one, two, ln, mass, *pool, keep=keep, first=4, last=30, key_pos=pos, kept=kept, work=ework, status=st)
+        N.evict_tokens(table, one, two, ln, mass, *pool, keep=keep, first=4, last=30, key_pos=pos, kept=whole, work=ework, status=st)        # all that is left of it
         for i in (0, 1):                                             # the next token of either row
             table[i + 1, keep] = fresh[i]
             pos[i + 1, keep].fill_(n)
