@@ -7,8 +7,13 @@
 // warps take 16 keys each, two tiles in turn, and come to the loaders' ring only through its barriers.
 //
 // Keys are the rows of the products (mma.sync, 16 x 8 x 16) and queries their eight columns: S^T = K Q^T and O^T += V^T P^T, so that the
-// four or eight heads of a group fill a fragment (as rows of sixteen they left half of every product and of the softmax idle: a tile of D = 64 took 1000 cycles of an SM
-// instead of the 700 its bytes take).  tcgen05 has no such narrow form: its 128 lanes would hold keys, and the softmax would run across lanes.
+// four or eight heads of a group fill a fragment (as rows of sixteen they left half of every product and of the softmax idle: heads of 256, 4 x 57,600 keys
+// 110 -> 96 us).  tcgen05 has no such narrow form: its 128 lanes would hold keys, and the softmax would run across lanes.  From 17 rows on
+// the products cost more than the cache: 36 rows (nine tokens of groups of four) take 2.7 times as long as four on the same keys.
+//
+// Microseconds on B200 (of them at the measured 6.54 TB/s): 4 x 57,600 keys, 8 KV heads of 128, groups of four: 154 (145); of 64: 91 (72); 2 heads of 256: 83 (72); with the
+// mass, 48 sequences of 600 to 9000 keys: 190 (147), two of 99,000 and 131,000: 185 (147); one sequence of 701 keys, heads of 64: 9.3, a launch, three dependent reads and a
+// join.  Rows of 512 bytes as bulk copies 96 -> 87, the cache's lines first out of L2 157 -> 154 and 196 -> 190 with the mass.
 //
 // Where a sequence ends inside a worker's part its state goes to the workspace, and the worker that comes last joins the
 // parts of a (sequence, KV head) in the order of its keys, so that results do not depend on the order of arrival.
@@ -23,7 +28,8 @@ namespace smc {
 constexpr int ST_FEW = 40, ST_MANY = 232;
 static_assert(128 * ST_FEW + 256 * ST_MANY <= 384 * 168, "the registers of the launch");
 constexpr int ST_MAX_BS = 1024, ST_LOADERS = 4;
-// Keys of a tile: what a loader warp does besides copying comes once a tile, and 64 keys of 128 bytes were too few to hide it (108 us against 4373 GB/s).
+// Keys of a tile: what a loader warp does besides copying comes once a tile, and 64 keys of 128 bytes were too few to hide it (4 x 57,600 keys of 8 heads of 64:
+// 108 us with tiles of 64 keys, 93 with 128).
 constexpr int step_tile(int D) { return D == 64 ? 128 : 64; }
 constexpr int ST_COUNTERS = 32768;                     // at the front of every workspace, whatever batch it serves next
 
@@ -638,7 +644,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
 }
 
 // mass[row, kvh, j] += sum over the rows of exp2(score - lse).  Every warp takes an equal run of tiles, a lane a key; four keys of a lane are in
-// flight at once (one tile after the other, each looked up anew, took 27 us for the 230,000 keys and 8 heads that take %s now).
+// flight at once (one tile after the other, each looked up anew: 27 us for 230,000 keys and 8 heads, 10 so, of them 4.5 at the memory's rate).
 constexpr int SM_WARPS = 8;
 
 __global__ void __launch_bounds__(SM_WARPS * 32) shaped_step_mass_kernel(const ShapedStepParams p) {

@@ -13,8 +13,8 @@ and a log-sum-exp of -inf.
 The cache is the block table's: one page per token, bf16 rows of Hkv * D values (the e4m3 cache is refused), all tokens of a call
 already written.  ``key_pos`` lists the positions of a row's tokens, ascending and below 2^24, once tokens have been shed; without it token j
 of a row has position j.  The weights live in ``mass`` [rows, Hkv, tokens], fp32, beside the block table; entries behind a row's last
-token are zero.  A key or value that is not finite spoils the tokens that share a tile of queries with one that sees it; tokens
-that nobody sees are not read.
+token are zero.  A key or value that is not finite spoils the tokens that share a tile of queries (up to 128 rows
+of tokens x heads) with one that sees it; cached tokens outside the span of a tile's intervals are not read.
 
 As everywhere, calls run on the current stream, allocate nothing and can be captured; ``status`` collects error bits.  Two calls that may
 run at the same time need a workspace each.
@@ -128,7 +128,7 @@ def attention_shaped_prompt(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
                             slopes: Optional[torch.Tensor] = None, bounds: Optional[torch.Tensor] = None, key_pos: Optional[torch.Tensor] = None,
                             lse: Optional[torch.Tensor] = None, pdl: bool = False) -> None:
     """Rotated queries ``q`` [T, Hq * D] of whole prompts or portions of them -> ``out`` [T, Hq * D] and ``lse`` [T, Hq].  ``runs`` [n, 4] int32 on the
-    device: block-table row, tokens held before, index of the first new token in ``q``, new tokens; rows of ``out`` that no run
+    device: block-table row, tokens held before, index of the first new token in ``q``, new tokens (no token of ``q`` in two runs); rows of ``out`` that no run
     names are left alone.  Heads of 64, 128 or 256, at most 128 query heads to a KV head."""
     L, dev, width = _library(), _device(q), Hkv * D
     (qp, ldq), (op, ldo) = _rows(q, "q", dev, T, Hq * D), _rows(out, "out", dev, T, Hq * D)

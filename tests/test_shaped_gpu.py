@@ -132,6 +132,27 @@ def test_prompt_attention_of_many_sequences_and_far_positions():
         _check(out, want, lse, want_lse, c, q, 8, 0.125, 20.0)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D", [(128, 1, 64), (100, 1, 128), (65, 1, 256), (66, 2, 64)])
+def test_groups_that_fill_or_miss_a_tile(Hq, Hkv, D):
+    """One token or two to a tile of rows, with rows left over."""
+    N = _N()
+    c = Cache([150, 3], Hkv, D, shed=True)
+    runs, T = [(1, 130, 0, 20), (2, 0, 20, 3)], 23
+    q, st = torch.randn(T, Hq * D, device=DEV).bfloat16(), _status()
+    want, want_lse, mass = attend(c, runs, q, Hq, scale=D ** -0.5, softcap=20.0, slopes=_slopes(Hq))
+    out, lse, m = torch.zeros(T, Hq * D, dtype=torch.bfloat16, device=DEV), torch.zeros(T, Hq, device=DEV), torch.zeros(3, Hkv, c.table.shape[1], device=DEV)
+    kw = dict(T=T, Hq=Hq, Hkv=Hkv, D=D, scale=D ** -0.5, status=st, softcap=20.0, slopes=_slopes(Hq), key_pos=c.key_pos)
+    r = torch.tensor(runs, dtype=torch.int32, device=DEV)
+    N.attention_shaped_prompt(q, c.k, c.v, c.table, r, out, lse=lse, **kw)
+    N.attention_key_mass(q, c.k, c.table, r, lse, m, **kw)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    _check(out, want, lse, want_lse, c, q, Hq, D ** -0.5, 20.0)
+    moved = _tolerances(c, q, Hq, D ** -0.5, 20.0)[1] * 2
+    for row, w in mass.items():
+        assert bool(((m[row, :, :w.shape[1]].double() - w).abs() <= moved * w + 2.0 ** -22 * (w + 1)).all())
+
+
 @pytest.mark.parametrize("slope", [0.9, -0.002])
 def test_distance_bias_against_opposed_scores(slope):
     """The highest scores lie far away and the distance takes them back (or adds to them): the reference must not bury the row."""
