@@ -265,6 +265,32 @@ def test_one_workspace_serves_batches_of_all_shapes():
             assert float((m[row, :, :w.shape[1]].double() / times - w).abs().max()) < 1e-4 * float(w.max())
 
 
+def test_calls_that_start_before_the_one_ahead_has_ended():
+    """The same bits with programmatic launches, each call reading what the one ahead of it writes."""
+    N = _N()
+    Hq, Hkv, D, n = 16, 4, 128, 700
+    c = Cache([n, 40], Hkv, D, shed=True)
+    q, st = torch.randn(n, Hq * D, device=DEV).bfloat16(), _status()
+    runs = torch.tensor([[1, 0, 0, n]], dtype=torch.int32, device=DEV)
+    work = torch.zeros(N.shaped_step_work_bytes(2, 1, Hq, Hkv, D, n + 40), dtype=torch.uint8, device=DEV)
+    rows, lens = torch.tensor([1, 2], device=DEV).int(), torch.tensor(c.lens, device=DEV).int()
+    got = []
+    for pdl in (False, True, True):
+        shape = dict(Hq=Hq, Hkv=Hkv, D=D, scale=D ** -0.5, status=st, softcap=30.0, slopes=_slopes(Hq), key_pos=c.key_pos, pdl=pdl)
+        out, lse, m = torch.zeros_like(q), torch.zeros(n, Hq, device=DEV), torch.zeros(3, Hkv, c.table.shape[1], device=DEV)
+        again, step = torch.zeros_like(q), torch.zeros(2, Hq * D, dtype=torch.bfloat16, device=DEV)
+        for _ in range(3):
+            N.attention_shaped_prompt(q, c.k, c.v, c.table, runs, out, T=n, lse=lse, **shape)
+            N.attention_key_mass(q, c.k, c.table, runs, lse, m, T=n, **shape)
+            N.attention_shaped_prompt(out, c.k, c.v, c.table, runs, again, T=n, **shape)
+            N.attention_shaped_step(again, c.k, c.v, c.table, rows, lens, step, bs=2, E=1, work=work, mass=m, **shape)
+        got.append((out, lse, m, again, step))
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    for other in got[1:]:
+        assert all(torch.equal(x, y) for x, y in zip(got[0], other))
+
+
 def test_bad_numbers_on_the_device_raise_the_status_and_read_nothing():
     N = _N()
     c = Cache([100, 100], 2, 64)
