@@ -41,7 +41,6 @@ struct ShapedMassParams {
 // What a step's query rows bring along, by column
 struct alignas(16) MsColumns {
   float neg_lse[MS_Q], pos[MS_Q], first[MS_Q], last[MS_Q], slope[MS_Q];
-  float reach[MS_Q];                                  // neg_lse and slope times the distance from the tile's first key: what a key in front of the token adds is linear
   float max_first[4], min_last[4], min_pos4[4];       // over 32 columns each: a key between the first two is seen by every column
 };
 
@@ -184,7 +183,6 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
     const int kvh = item % p.Hkv, hbase = kvh * G, keys = run.held + run.n, k0 = tile * NT * 128;
     const int* kp = p.c.key_pos != nullptr ? p.c.key_pos + (size_t)run.row * p.c.kp_stride : nullptr;
     auto pos_of = [&](int idx) { return kp != nullptr ? kp[idx] : idx; };
-    const float base_pos = BIAS && have ? (float)pos_of(k0) : 0.f;
     // new tokens [ta, tb) of the run that may see one of the keys
     int ta = max(0, k0 - run.held), tb = have ? run.n : 0;
     if (p.c.bounds != nullptr) {
@@ -265,10 +263,7 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         col.pos[cl] = posf;
         col.first[cl] = first;
         col.last[cl] = last;
-        if (BIAS) {
-          col.slope[cl] = slope;
-          col.reach[cl] = nl + slope * (posf - base_pos);
-        }
+        if (BIAS) col.slope[cl] = slope;
         const float mf = warp_max(first), ml = -warp_max(-last);
         const float mp = BIAS ? -warp_max(live ? -posf : -(float)SH_POS_END) : 0.f;
         if (lane == 0) { col.max_first[lw] = mf; col.min_last[lw] = ml; col.min_pos4[lw] = mp; }
@@ -331,7 +326,7 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
       const uint32_t ts = tmem_base + (uint32_t)t * 256u + (((uint32_t)((warp & 3) * 32)) << 16);
       const float kpos = k < keys ? (float)pos_of(k) : -1.f;
       const float mul = p.c.mul, cap_in = p.c.cap_in, cap_out = p.c.cap_out;
-      const uint64_t mul2 = f2_pair(mul, mul), kpos2 = f2_pair(kpos, kpos), from_base2 = f2_pair(base_pos - kpos, base_pos - kpos);
+      const uint64_t mul2 = f2_pair(mul, mul), ahead2 = f2_pair(-kpos, -kpos);
       const ShapedCapNear<4> near(cap_in, cap_out, mul);
       float* to = p.mass + ((size_t)run.row * p.Hkv + kvh) * p.mass_stride + k;
       const float before = C == 1 && k < keys ? *to : 0.f;          // long back when the sum is there
@@ -351,20 +346,18 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
           constexpr bool PLAIN = decltype(plain)::value;
 #pragma unroll
           for (int i = 0; i < 32; i += 4) {
-            const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(BIAS && PLAIN ? &col.reach[c0 + i] : &col.neg_lse[c0 + i]);
+            const ulonglong2 nl = *reinterpret_cast<const ulonglong2*>(&col.neg_lse[c0 + i]);
             uint64_t off[2] = {nl.x, nl.y};
-            if (BIAS) {
-              const ulonglong2 sl = *reinterpret_cast<const ulonglong2*>(&col.slope[c0 + i]);
-              if constexpr (PLAIN) {
-                off[0] = f2_fma(from_base2, sl.x, off[0]);
-                off[1] = f2_fma(from_base2, sl.y, off[1]);
-              } else {
-                const ulonglong2 at = *reinterpret_cast<const ulonglong2*>(&col.pos[c0 + i]);
+            if (BIAS) {                               // (the distance itself first, exact: shares of it from some point between would cancel across a gap in the positions)
+              const ulonglong2 sl = *reinterpret_cast<const ulonglong2*>(&col.slope[c0 + i]), at = *reinterpret_cast<const ulonglong2*>(&col.pos[c0 + i]);
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                  const float2 v = f2_unpair(f2_fma(kpos2, f2_pair(-1.f, -1.f), k ? at.y : at.x));
-                  off[k] = f2_fma(f2_pair(fabsf(v.x), fabsf(v.y)), k ? sl.y : sl.x, off[k]);
+              for (int k = 0; k < 2; ++k) {
+                uint64_t far = f2_add(k ? at.y : at.x, ahead2);
+                if constexpr (!PLAIN) {
+                  const float2 v = f2_unpair(far);
+                  far = f2_pair(fabsf(v.x), fabsf(v.y));
                 }
+                off[k] = f2_fma(far, k ? sl.y : sl.x, off[k]);
               }
             }
 #pragma unroll

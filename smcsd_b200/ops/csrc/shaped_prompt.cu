@@ -55,8 +55,8 @@ struct ShapedPromptParams {
 template <int D> struct SpShared {
   static constexpr int SLOTS = SpCfg<D>::UNITS / 2 + 1;               // steps whose keys' positions are held
   uint64_t kv_full[SpCfg<D>::UNITS], kv_empty[SpCfg<D>::UNITS], q_full[2], s_full[2][2], p_full[2][2][2], o_done[2][2], pos_full[SLOTS], turn[2][4];
-  alignas(16) float pos[SLOTS][SpCfg<D>::BK];         // of a step's keys, less that of the first; SP_NONE behind the last
-  float pos_first[SLOTS];
+  alignas(16) float pos[SLOTS][SpCfg<D>::BK];         // of a step's keys, less that of the first or, with distances, of the one nearest the tile's tokens; SP_NONE behind the last
+  float pos_near[SLOTS];
   uint32_t tmem_slot;
   int lo[8], hi[8], begin, end[2];
   volatile int abort;
@@ -252,16 +252,17 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
     constexpr int LAG = 1, PD = 2;                     // gathered units in flight behind the newest (a unit is handed over LAG later, when as many more slots are free); steps that page ids are read ahead
     int issued = 0;
     uint32_t gathered = 0;                            // bit (u & 31): this warp's part of unit u went through cp.async (arrival still owed)
-    int pg[PD][KL], pk[PD], p0[PD];
-    auto ahead = [&](int step, int (&ids)[KL], int& pos, int& first_pos) {
+    int pg[PD][KL], pk[PD], pn[PD];
+    auto ahead = [&](int step, int (&ids)[KL], int& pos, int& near_pos) {
 #pragma unroll
       for (int i = 0; i < KL; ++i) ids[i] = step < n_steps ? bt[min(begin + step * BK + i * 32 + lane, end_all - 1)] : 0;
-      const int k = begin + step * BK + lw * KPW + lane, k0 = begin + step * BK;      // the positions this warp hands over
+      const int k0 = begin + step * BK, k = k0 + lw * KPW + lane;      // the positions this warp hands over
       pos = lane < KPW && k < end_all ? (kp != nullptr ? kp[k] : k) : -1;
-      first_pos = k0 < end_all ? (kp != nullptr ? kp[k0] : k0) : 0;
+      const int k_near = !BIAS || k0 >= first ? k0 : min(k0 + BK, end_all) - 1;  // keys in front of the tile's tokens: the last one
+      near_pos = k0 < end_all ? (kp != nullptr ? kp[k_near] : k_near) : 0;
     };
 #pragma unroll
-    for (int d = 0; d < PD; ++d) ahead(d, pg[d], pk[d], p0[d]);
+    for (int d = 0; d < PD; ++d) ahead(d, pg[d], pk[d], pn[d]);
     bool go = true;
     const uint64_t pol = l2_policy_evict_last();      // the other row tiles of this KV head read the same keys
     for (int j0 = 0; go && j0 < n_steps; j0 += PD) {
@@ -272,8 +273,8 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
         int page[KL];
 #pragma unroll
         for (int i = 0; i < KL; ++i) page[i] = checked(pg[d][i]);
-        const float pos = pk[d] < 0 ? SP_NONE : (float)(pk[d] - p0[d]), pos_first = (float)p0[d];
-        ahead(j + PD, pg[d], pk[d], p0[d]);
+        const float pos = pk[d] < 0 ? SP_NONE : (float)(pk[d] - pn[d]), pos_near = (float)pn[d];
+        ahead(j + PD, pg[d], pk[d], pn[d]);
         int base[KL / 2];
         bool rows_run[KL / 2];
 #pragma unroll
@@ -291,7 +292,7 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
           if (!__all_sync(0xffffffffu, ok)) { go = false; break; }
           if (kv == 0) {                              // the ring of positions turns with the keys
             if (lane < KPW) S.pos[j % SLOTS][lw * KPW + lane] = pos;
-            if (lw == 0 && lane == 0) S.pos_first[j % SLOTS] = pos_first;
+            if (lw == 0 && lane == 0) S.pos_near[j % SLOTS] = pos_near;
             __syncwarp();
             if (lane == 0) mbar_arrive(&S.pos_full[j % SLOTS]);
           }
@@ -433,6 +434,23 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
       tc_fence_after();
       const float* pos = S.pos[j % SLOTS];
       const uint32_t ts = tmem_base + (uint32_t)((t * SB + j % SB) * BK) + lane_off;
+      // Where the step lies, ahead of its scores where distances make this longer.  Its keys ascend, those behind the last (position -1) come at its end.
+      float nearest, pos0, pos1;
+      bool plain, behind = false;
+      auto place = [&] {
+        nearest = S.pos_near[j % SLOTS];
+        pos0 = BIAS ? nearest + pos[0] : nearest;
+        pos1 = nearest + pos[BK - 1];
+        bool mine = pos0 >= first_seen && pos1 >= 0.f && pos1 <= last_seen;
+        if (BIAS) {
+          // A distance is linear over the step from its nearest key on; taken from the farthest one, beyond a gap in the positions, the near ones would be differences of
+          // large numbers.  So the row has to lie beyond that key (one inside the step looks both ways), and where far keys gain the step has to be short.
+          behind = nearest == pos1;
+          mine = mine && (slope == 0.f || (behind ? pos_row >= pos1 : pos_row <= pos0)) && slope * (pos1 - pos0) <= 16.f;
+        }
+        plain = __all_sync(0xffffffffu, mine);
+      };
+      if (BIAS) place();
       uint32_t x[BK];
 #pragma unroll
       for (int c0 = 0; c0 < BK; c0 += 16) tmem_ld_32x32b_x16(ts + c0, *reinterpret_cast<uint32_t(*)[16]>(&x[c0]));
@@ -452,13 +470,10 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
         }
       }
       const float most = fmaxf(mx[0], mx[1]), least = fminf(mn[0], mn[1]), reach = fmaxf(most, -least) * cap_in;
-      // the keys of a step ascend, those behind the last (position -1) come at its end
-      const float pos0 = S.pos_first[j % SLOTS], pos1 = pos0 + pos[BK - 1];
-      const bool full = __all_sync(0xffffffffu, pos0 >= first_seen && pos1 >= 0.f && pos1 <= last_seen);
+      if (!BIAS) place();
       // 0: scores as they are after this; 1: tanh by three coefficients (or none); 2: by five
       int way = 1;
-      // (a row whose own position lies inside the step looks both ways)
-      if (!full || (BIAS && __any_sync(0xffffffffu, !((most - least) * mul < 60.f) || (pos0 < pos_row && pos1 > pos_row)))) way = 0;
+      if (!plain || (BIAS && __any_sync(0xffffffffu, !((most - least) * mul < 60.f)))) way = 0;
       else if (CAP && __any_sync(0xffffffffu, !(reach <= near.reach))) way = __any_sync(0xffffffffu, !(reach <= SH_TANH5_REACH)) ? 0 : 2;
       float top;
       if (way != 0) {
@@ -484,7 +499,7 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
         top = -INFINITY;
 #pragma unroll
         for (int i = 0; i < BK; ++i) {
-          const float at = pos0 + pos[i];
+          const float at = nearest + pos[i];
           float v = val(i);
           if (BIAS) v = fmaf(fabsf(at - pos_row), slope, v);
           v = at >= first_seen && at <= last_seen ? v : -INFINITY;    // probability zero
@@ -546,8 +561,8 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
         }
       };
       const uint64_t mul2 = f2_pair(mul, mul), off = f2_pair(-ref, -ref);
-      // distance's share less the reference: linear over the step, from its first key on
-      const float per = pos0 < pos_row ? -slope : slope, start = slope * fabsf(pos0 - pos_row) - ref;
+      // distance's share less the reference, from the nearest key on
+      const float per = behind ? -slope : slope, start = fmaf(slope, fabsf(nearest - pos_row), -ref);
       const uint64_t per2 = f2_pair(per, per), start2 = f2_pair(start, start);
       auto away = [&](int i) {
         if (!BIAS) return off;

@@ -1,0 +1,99 @@
+"""Shaped attention where caches, masks and numbers are at their edges, on the GPU against float64 (shaped_oracle.py)."""
+import math
+
+import pytest
+import torch
+
+from shaped_oracle import Cache, attend
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _N():
+    from smcsd_b200.ops import native_shaped as N
+    return N
+
+
+def _int(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _slopes(Hq):
+    return torch.tensor([2.0 ** (-8.0 * (h + 1) / Hq) for h in range(Hq)], device=DEV)
+
+
+def _randn(*shape, seed=0):
+    """bf16 from a generator of its own: the default one's order belongs to the other tests."""
+    return torch.randn(*shape, device=DEV, generator=torch.Generator(DEV).manual_seed(seed)).bfloat16()
+
+
+def _out_error(c, moved):
+    """An output's: every probability and the output itself are rounded to bf16, by 2^-8 of themselves at most (half a step), and a score's error moves a probability by as much,
+    against the sum of all once more."""
+    return (2 * 2.0 ** -8 + 2 * moved) * float(c.v[1:].double().abs().max())
+
+
+def _score_error(c, q, scale):
+    """How far a score may be off: products of D values summed in fp32, every addition by at most 2^-23 of the largest partial sum, |q||k| scale."""
+    big = float((q.double().view(-1, c.D).norm(dim=1).max() * c.k[1:].double().view(-1, c.D).norm(dim=1).max()) * scale)
+    return c.D / 16 * 2.0 ** -23 * big
+
+
+# ------------------------------------------------------------------------------- gaps in the positions
+def _gap_cache(lens, Hkv, D, ahead, gap, seed):
+    """Rows of which ``ahead`` tokens lie at the front, the others ``gap`` positions further on."""
+    c = Cache(lens, Hkv, D, seed=seed, order="up", shed=True)
+    at = torch.arange(c.table.shape[1], device=DEV)
+    c.key_pos[:] = at + gap * (at >= ahead)
+    return c
+
+
+@pytest.mark.parametrize("gap", [6 * 10 ** 4, 10 ** 6, 2 ** 24 - 2000])
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 64), (16, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("softcap", [0.0, 30.0])
+def test_distance_bias_across_a_gap_inside_a_step(gap, Hq, Hkv, D, softcap):
+    """Held tokens fill whole steps of keys, of which the first ones lie far in front of the rest: the distances of the near ones must not drown in those.  A weight is off by
+    what the score is, the log-sum-exp by that and half a unit in the last place of an fp32 number of its size (2^-20 covers numbers up to 16)."""
+    N = _N()
+    held, n = 512, 40
+    for ahead in (8, 500):
+        c = _gap_cache([held + n, held], Hkv, D, ahead, gap, seed=gap % 97 + ahead)
+        runs = [(1, held, 0, n)]
+        q, st = _randn(n, Hq * D, seed=gap + D), _int([0])
+        kw = dict(scale=D ** -0.5, softcap=softcap, slopes=_slopes(Hq))
+        want, want_lse, mass = attend(c, runs, q, Hq, **kw)
+        out, lse, m = torch.zeros_like(q), torch.zeros(n, Hq, device=DEV), torch.zeros(3, Hkv, c.table.shape[1], device=DEV)
+        kw.update(T=n, Hq=Hq, Hkv=Hkv, D=D, status=st, key_pos=c.key_pos)
+        N.attention_shaped_prompt(q, c.k, c.v, c.table, _int(runs), out, lse=lse, **kw)
+        N.attention_key_mass(q, c.k, c.table, _int(runs), want_lse.float(), m, **kw)
+        torch.cuda.synchronize()
+        assert int(st) == 0
+        moved = _score_error(c, q, D ** -0.5) + 3e-6 * (softcap or 0.0) + 2.0 ** -20
+        assert float((lse.double() - want_lse).abs().max()) <= moved
+        assert float((out.double().view(want.shape) - want).abs().max()) <= _out_error(c, moved)
+        w = mass[1]
+        # weights far below a key's sum may be rounded away: the bias of a far key is as large as its distance, and so is its rounding, but exp of it is nothing
+        assert bool(((m[1, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
+
+
+@pytest.mark.parametrize("slope", [-0.002, -0.3])
+def test_distance_bias_that_grows_across_a_gap(slope):
+    """A negative slope favours the far tokens: those at the other end of the step have to be right then.  Scores grow with the distance and so does what fp32 can tell of
+    them: half a unit of the largest, once for the product and once for the sum, in the score and in the reference."""
+    N = _N()
+    held, n, Hq, D, gap = 256, 30, 4, 64, 5000
+    c = _gap_cache([held + n], 1, D, 100, gap, seed=3)
+    runs, slopes = [(1, held, 0, n)], torch.full((Hq,), slope, device=DEV)
+    q, st = _randn(n, Hq * D, seed=gap + D), _int([0])
+    want, want_lse, mass = attend(c, runs, q, Hq, scale=0.125, slopes=slopes)
+    out, lse, m = torch.zeros_like(q), torch.zeros(n, Hq, device=DEV), torch.zeros(2, 1, c.table.shape[1], device=DEV)
+    kw = dict(scale=0.125, slopes=slopes, T=n, Hq=Hq, Hkv=1, D=D, status=st, key_pos=c.key_pos)
+    N.attention_shaped_prompt(q, c.k, c.v, c.table, _int(runs), out, lse=lse, **kw)
+    N.attention_key_mass(q, c.k, c.table, _int(runs), lse, m, **kw)
+    torch.cuda.synchronize()
+    moved = _score_error(c, q, 0.125) + 4 * 2.0 ** -24 * -slope * (gap + held + n) * 1.5 + 2.0 ** -20
+    assert int(st) == 0 and float((lse.double() - want_lse).abs().max()) <= moved
+    assert float((out.double().view(want.shape) - want).abs().max()) <= _out_error(c, moved)
+    w = mass[1]
+    assert bool(((m[1, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
