@@ -25,6 +25,12 @@ struct ShapedCache {
   float cap_in, cap_out;         // scale / cap and cap log2(e), 0: no cap
 };
 
+// Scales and caps (0: none) whose factors are fp32 numbers: scale log2(e), scale / cap and cap log2(e).
+inline bool shaped_scores_fit(float scale, float cap) {
+  auto normal = [](double x) { return x >= 1.2e-38 && x <= 3.4e38; };
+  return normal((double)scale * 1.4426950408889634) && (cap == 0.f || (cap > 0.f && normal((double)scale / cap) && normal((double)cap * 1.4426950408889634)));
+}
+
 // (in double precision: an error of a factor is one of every score)
 inline ShapedCache shaped_cache(const int* block_table, int bt_stride, int bt_rows, int n_pages, const int* key_pos, int kp_stride, const int* bounds,
                                 const float* slopes, float scale, float cap) {
@@ -160,8 +166,8 @@ __device__ __forceinline__ float shaped_cap(float x, float in, float out) {
   }
   return t * out;
 }
-// out tanh(x in) + add of two numbers within reach.  With three or four coefficients the factors are folded into them (N + 1 operations a pair); the
-// powers of `in` stay in range of fp32 for in >= 2e-5, below that the reach is nothing.  With more, u is made first.
+// out tanh(x in) + add of two numbers within reach.  With three or four coefficients the factors are folded into them (N + 1 operations a pair); where the
+// powers of `in` leave the range of fp32 the reach is nothing, not even zero.  With more, u is made first.
 template <int N>
 struct ShapedCapNear {
   uint64_t c[N], in2;
@@ -174,7 +180,7 @@ struct ShapedCapNear {
       if (N <= 4) f *= in * in;
     }
     in2 = f2_pair(in, in);
-    reach = N <= 4 ? (in >= 2e-5f ? SH_TANH3_REACH : -1.f) : N == 5 ? SH_TANH5_REACH : SH_TANH6_REACH;
+    reach = N <= 4 ? (in >= 2e-5f && f <= 1e38f ? SH_TANH3_REACH : -1.f) : N == 5 ? SH_TANH5_REACH : SH_TANH6_REACH;
   }
   __device__ __forceinline__ uint64_t operator()(uint64_t x, uint64_t add) const {
     const uint64_t u = N <= 4 ? x : f2_mul(x, in2), y = f2_mul(u, u);

@@ -474,7 +474,7 @@ SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, i
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(runs)) & 15 || (ld_q & 7) || ld_q > (1 << 23) ||
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -161;
-  if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -162;
+  if (!shaped_scores_fit(scale, cap)) return -162;
   if (mass_stride < bt_stride) return -163;
   ShapedMassParams p;
   p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);

@@ -657,7 +657,7 @@ SMC_API int smc_shaped_prompt(const void* q, long long ld_q, const void* k_pool,
        reinterpret_cast<uintptr_t>(v_pool)) & 15)
     return -141;
   if ((ld_q & 7) || (ld_out & 7) || (reinterpret_cast<uintptr_t>(bounds) & 7)) return -142;
-  if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -143;
+  if (!shaped_scores_fit(scale, cap)) return -143;
   ShapedPromptParams p;
   p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.v_pool = (const __nv_bfloat16*)v_pool;

@@ -773,7 +773,7 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
       ((reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) || (reinterpret_cast<uintptr_t>(work) & 15) ||
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -151;
-  if (!(cap >= 0.f) || cap > 3e38f || !(scale > 0.f) || scale > 3e38f) return -152;
+  if (!shaped_scores_fit(scale, cap)) return -152;
   if (mass != nullptr && mass_stride < bt_stride) return -153;
   StepWork w = step_work(bs, E, Hq, Hkv, D, 0);
   if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hkv * ((E * (Hq / Hkv) + 3) / 4 * 4) * step_tile(D) * 4);       // the rest of it

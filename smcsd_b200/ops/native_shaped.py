@@ -3,7 +3,7 @@
 With x = scale q.k, then ``softcap`` tanh(x / softcap) where ``softcap`` > 0, then x - slopes[head] |distance| where ``slopes`` are given,
 a token attends the cached tokens whose positions lie in its interval ``bounds[t]`` = (first, last), both included; without
 ``bounds`` all up to its own.  ``score_bounds`` makes the intervals of windows, packed documents and prefixes.  A token that sees nothing gets zeros
-and a log-sum-exp of -inf.
+and a log-sum-exp of -inf.  ``scale``, ``softcap`` and ``scale / softcap`` have to lie within the range of normal fp32 numbers, or the call is refused.
 
     attention_shaped_prompt    many tokens of a sequence
     attention_shaped_step      the last one or few of each

@@ -1,0 +1,19 @@
+"""Shaped attention at its edges, as far as that goes without a GPU."""
+import os
+
+import pytest
+
+from smcsd_b200.ops import native as K
+from smcsd_b200.ops import native_shaped as N
+
+needs_library = pytest.mark.skipif(not os.path.exists(os.path.join(os.path.dirname(K.__file__), "libsmcsd_b200.so")), reason="kernel library not built")
+
+
+@needs_library
+@pytest.mark.parametrize("scale,cap", [(0.125, 1e-42), (0.125, 3e38), (0.125, 1e38), (1e30, 1e-10), (3e38, 0.0), (1e-40, 0.0), (1e-30, 1e9), (0.0, 5.0), (float("inf"), 5.0), (0.125, float("nan"))])
+def test_scales_and_caps_outside_of_fp32_are_refused_ahead_of_any_launch(scale, cap):
+    """scale log2(e), scale / cap or cap log2(e) is not a normal fp32 number."""
+    L, p = N._library(), 1 << 20
+    assert L.smc_shaped_prompt(p, 512, p, p, 7, p, 8, 1, None, 0, p, 1, p, 512, None, 4, 8, 2, 64, scale, cap, None, None, p, 0, None) == -143
+    assert L.smc_shaped_mass(p, 512, p, 7, p, 8, 1, None, 0, p, 1, p, p, 8, 4, 8, 2, 64, scale, cap, None, None, p, 0, None) == -162
+    assert L.smc_shaped_step(p, 512, p, p, 7, p, 8, 1, None, 0, p, p, p, 512, None, None, 8, 2, 1, 8, 2, 64, scale, cap, None, None, p, 1 << 30, p, 0, None) == -152

@@ -97,3 +97,34 @@ def test_distance_bias_that_grows_across_a_gap(slope):
     assert float((out.double().view(want.shape) - want).abs().max()) <= _out_error(c, moved)
     w = mass[1]
     assert bool(((m[1, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
+
+
+# ------------------------------------------------------------------------------- caps far below and above the scores
+@pytest.mark.parametrize("cap", [1e-30, 1e-8, 1e-6, 1e-3, 1e5, 1e30])
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (8, 2, 128), (8, 2, 256)])
+def test_caps_far_from_the_scores(cap, Hq, Hkv, D):
+    """Scores of zero too: a key tile, a row of tokens and a whole sequence of them beside ordinary ones.  A capped score is off by 3e-6 of itself, an uncapped one by its
+    product's error."""
+    N = _N()
+    c = Cache([300, 150], Hkv, D, seed=2)
+    q, st = _randn(450, Hq * D, seed=8), _int([0])
+    q[40:170] = 0
+    q[300:] = 0
+    c.k[c.table[1, 128:256].long()] = 0
+    runs, scale = [(1, 0, 0, 300), (2, 0, 300, 150)], D ** -0.5
+    want, want_lse, mass = attend(c, runs, q, Hq, scale=scale, softcap=cap)
+    out, lse, m = torch.zeros_like(q), torch.zeros(450, Hq, device=DEV), torch.zeros(3, Hkv, c.table.shape[1], device=DEV)
+    kw = dict(Hq=Hq, Hkv=Hkv, D=D, scale=scale, softcap=cap, status=st)
+    N.attention_shaped_prompt(q, c.k, c.v, c.table, _int(runs), out, T=450, lse=lse, **kw)
+    N.attention_key_mass(q, c.k, c.table, _int(runs), lse, m, T=450, **kw)
+    work = torch.zeros(N.shaped_step_work_bytes(2, 1, Hq, Hkv, D), dtype=torch.uint8, device=DEV)
+    out1, lse1 = torch.zeros(2, Hq * D, dtype=torch.bfloat16, device=DEV), torch.zeros(2, Hq, device=DEV)
+    N.attention_shaped_step(q[[299, 449]], c.k, c.v, c.table, _int([1, 2]), _int([300, 150]), out1, bs=2, E=1, work=work, lse=lse1, **kw)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    moved = _score_error(c, q, scale) + 3e-6 * min(cap, 30.0) + 2.0 ** -20
+    for o, l, at in ((out, lse, slice(None)), (out1, lse1, [299, 449])):
+        assert float((o.double().view(-1, Hq, D) - want[at]).abs().max()) <= _out_error(c, moved)
+        assert float((l.double() - want_lse[at]).abs().max()) <= moved
+    for row, w in mass.items():
+        assert bool(((m[row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
