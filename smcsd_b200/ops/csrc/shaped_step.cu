@@ -653,13 +653,14 @@ __global__ void __launch_bounds__(SM_WARPS * 32) shaped_step_mass_kernel(const S
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, G = p.Hq / p.Hkv, M = p.E * G, pitch = (M + 3) / 4 * 4;
   step_schedule(p, sm_tiles, sm_tiles + p.bs + 1);                   // from what was there before the first kernel
   const int total = sm_tiles[p.bs], many = gridDim.x * SM_WARPS, me = blockIdx.x * SM_WARPS + warp;
+  // on every path: whoever follows waits for this grid alone, which must not end ahead of the first kernel
+  pdl_wait_prior_grid();
   if (total > p.score_tiles) {                                       // the workspace is too small for these contexts
     if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(p.status, SMC_ERR_BOUNDS);
     return;
   }
   const int x_end = step_first(me + 1, many, total);
   int x = step_first(me, many, total);
-  pdl_wait_prior_grid();
   while (x < x_end) {
     StepCursor cur;
     cur.seek(p, sm_tiles, x);

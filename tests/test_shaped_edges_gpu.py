@@ -128,3 +128,45 @@ def test_caps_far_from_the_scores(cap, Hq, Hkv, D):
         assert float((l.double() - want_lse[at]).abs().max()) <= moved
     for row, w in mass.items():
         assert bool(((m[row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
+
+
+# ------------------------------------------------------------------------------- a workspace that contexts have outgrown
+def test_step_behind_one_whose_workspace_was_too_small():
+    """The refused weights raise the status; the step's outputs are there for whoever comes next, also for one that starts early, and the workspace is fit for the next step."""
+    N = _N()
+    Hq, Hkv, D = 8, 2, 64
+    c = Cache([9000, 8000], Hkv, D, seed=4)
+    q, st = _randn(2, Hq * D, seed=5), _int([0])
+    rows, lens = _int([1, 2]), _int(c.lens)
+    want, _, mass = attend(c, [(1, 8999, 0, 1), (2, 7999, 1, 1)], q, Hq, scale=0.125)
+    tol = _out_error(c, _score_error(c, q, 0.125) + 2.0 ** -20)
+    small = N.shaped_step_work_bytes(2, 1, Hq, Hkv, D, 300)
+    work = torch.zeros(N.shaped_step_work_bytes(2, 1, Hq, Hkv, D, 17000), dtype=torch.uint8, device=DEV)
+    outs = [torch.zeros_like(q) for _ in range(8)]
+    m = [torch.zeros(3, Hkv, c.table.shape[1], device=DEV) for _ in range(2)]
+    kw = dict(bs=2, E=1, Hq=Hq, Hkv=Hkv, D=D, scale=0.125, status=st)
+
+    def chain():
+        for i in range(0, 8, 2):
+            N.attention_shaped_step(q, c.k, c.v, c.table, rows, lens, outs[i], work=work[:small], mass=m[0], **kw)
+            N.attention_shaped_step(outs[i], c.k, c.v, c.table, rows, lens, outs[i + 1], work=work, pdl=True, **kw)
+    chain()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        chain()
+    g.replay()
+    torch.cuda.synchronize()
+    assert int(st) == 8 and not bool(m[0].any())
+    again, _, _ = attend(c, [(1, 8999, 0, 1), (2, 7999, 1, 1)], outs[0], Hq, scale=0.125)
+    for i in range(0, 8, 2):
+        assert torch.equal(outs[i], outs[0]) and torch.equal(outs[i + 1], outs[1])
+    assert float((outs[0].double().view(want.shape) - want).abs().max()) <= tol
+    assert float((outs[1].double().view(want.shape) - again).abs().max()) <= tol
+    st.zero_()
+    N.attention_shaped_step(q, c.k, c.v, c.table, rows, lens, outs[0], work=work, mass=m[1], **kw)
+    torch.cuda.synchronize()
+    assert int(st) == 0 and torch.equal(outs[0], outs[2])
+    for row, w in mass.items():
+        moved = _score_error(c, q, 0.125) + 2.0 ** -20
+        assert bool(((m[1][row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
