@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
   int* counter = p.counters + kvh;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&S.full[i], Cfg::BULK ? ST_LOADERS : ST_LOADERS * 32);
+      mbar_init(&S.full[i], Cfg::BULK ? ST_LOADERS : ST_LOADERS * (p.c.key_pos != nullptr ? 33 : 32));
       mbar_init(&S.empty[i], Cfg::GW * MT);
     }
     S.abort = 0;
@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
             st_cp16(to + (uint32_t)(r * LD * 2), from_k + off, policy);
             st_cp16(to + (uint32_t)(r * LD * 2) + (uint32_t)Cfg::KV, from_v + off, policy);
           }
-          __syncwarp();                                              // each lane arrives once its own copies have landed
+          __syncwarp();                                              // each lane arrives once its own copies have landed, which says nothing of positions
+          if (kp != nullptr && lane == 0) mbar_arrive(&S.full[st]);
           asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(&S.full[st])) : "memory");
         }
         --left;

@@ -170,3 +170,36 @@ def test_step_behind_one_whose_workspace_was_too_small():
     for row, w in mass.items():
         moved = _score_error(c, q, 0.125) + 2.0 ** -20
         assert bool(((m[1][row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
+
+
+# ------------------------------------------------------------------------------- listed positions
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 64), (16, 4, 128), (16, 2, 256)])
+def test_listed_positions_are_there_when_their_keys_are(Hq, Hkv, D):
+    """A hundred replays of a step whose masks and distances rest on listed positions, caches and positions changing place between them: the same bits as at first."""
+    N = _N()
+    lens = [2500, 700, 64, 3000]
+    c = Cache(lens, Hkv, D, seed=6, shed=True)
+    q, st = _randn(4, Hq * D, seed=7), _int([0])
+    work = torch.zeros(N.shaped_step_work_bytes(4, 1, Hq, Hkv, D), dtype=torch.uint8, device=DEV)
+    own = torch.stack([c.key_pos[i + 1, n - 1] for i, n in enumerate(lens)])
+    bounds, slopes, scale = N.score_bounds(own, window=900), _slopes(Hq), D ** -0.5
+    want, _, _ = attend(c, [(i + 1, n - 1, i, 1) for i, n in enumerate(lens)], q, Hq, scale=scale, slopes=slopes, bounds=bounds)
+    out, other = torch.zeros_like(q), torch.zeros_like(q)
+    kw = dict(bs=4, E=1, Hq=Hq, Hkv=Hkv, D=D, scale=scale, status=st, work=work, slopes=slopes)
+    g = torch.cuda.CUDAGraph()
+    far = c.key_pos + 5
+
+    def step(o, pos):
+        N.attention_shaped_step(q, c.k, c.v, c.table, _rows, _lens, o, bounds=bounds if pos is c.key_pos else shifted, key_pos=pos, **kw)
+    _rows, _lens, shifted = _int([1, 2, 3, 4]), _int(lens), bounds + 5
+    step(out, c.key_pos)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        step(other, far)                                             # the same distances and masks
+        step(out, c.key_pos)
+    first = out.clone()
+    assert float((first.double().view(want.shape) - want).abs().max()) <= _out_error(c, _score_error(c, q, scale) + 2.0 ** -20)
+    for _ in range(100):
+        g.replay()
+        assert torch.equal(out, first)
+    assert torch.equal(other, first) and int(st) == 0
