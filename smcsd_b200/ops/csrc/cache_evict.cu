@@ -13,7 +13,7 @@
 // What bounds it: 4 bytes per token and head read once, then barriers and dependent reads; the row that takes longest decides.  (In one kernel, the moves of a cluster
 // kept in step by barriers between heads: 115 us for 16 rows of 65,000 tokens and 8 heads from two sources, 50 so; 16 rows of 2,100
 // tokens 26: reads of the weights 5, three histograms 5, places 4, moves 5, launches.)
-#include "common.cuh"
+#include "shaped.cuh"
 
 namespace smc {
 
@@ -37,7 +37,7 @@ struct EvictParams {
   unsigned* bits;
   int* old;                                            // [EV_ENTRIES] what the second kernel has to know: the row's length before, -1: leave it alone
   long long bt_stride, kp_stride, mass_stride;
-  int n_rows, rows, heads, n_pages, keep, first, last, capacity;
+  int cols, n_rows, rows, heads, n_pages, keep, first, last, capacity;
   int* status;
 };
 
@@ -95,9 +95,9 @@ __global__ void __launch_bounds__(EV_T, 2) evict_kernel(const EvictParams p) {
   shared = __syncthreads_or(shared);
   int n = src >= 0 && src < p.rows ? p.lens[src] : -1;
   const int old = fine ? p.lens[dst] : 0;
-  const bool known = n >= 0 && n <= p.bt_stride;       // (an entry that clashes still answers for those that share its source)
+  const bool known = n >= 0 && n <= p.cols;            // (an entry that clashes still answers for those that share its source)
   n = known ? n : 0;
-  fine = fine && known && old >= 0 && old <= p.bt_stride;
+  fine = fine && known && old >= 0 && old <= p.cols;
   const bool solo = n <= EV_SOLO, in_place = src == dst;
   const int CL = solo ? 1 : EV_CL;
   auto barrier = [&] { if (solo) __syncthreads(); else cluster_sync(); };
@@ -360,24 +360,25 @@ __global__ void __launch_bounds__(EV_T) evict_move_kernel(const EvictParams p) {
 // Bytes of workspace (zeros at first) for an allocator of n_pages pages.
 SMC_API long long smc_evict_work(int n_pages) { return n_pages < 1 ? -1 : 256 + smc::EV_ENTRIES * 4 + ((long long)n_pages / 32 + 1) * 4; }
 
-// src, dst [n_rows] int32 rows of table [rows, bt_stride], key_pos [rows, kp_stride] or null and mass [rows, heads, mass_stride] fp32, with lens [rows]; a
+// src, dst [n_rows] int32 rows of table [rows, columns], key_pos [rows, kp_stride] or null and mass [rows, heads, mass_stride] fp32, with lens [rows]; a
 // row is written by one entry at most and then read by no other.  kept [n_rows, keep].
-SMC_API int smc_evict(int* table, long long bt_stride, int* key_pos, long long kp_stride, float* mass, long long mass_stride, int* lens, int rows,
+SMC_API int smc_evict(int* table, long long bt_pitch, int* key_pos, long long kp_stride, float* mass, long long mass_stride, int* lens, int rows,
                       const int* src, const int* dst, int n_rows, int heads, int keep, int first, int last, int* kept, int* refcount, int* free_stack,
                       int* free_count, int n_pages, void* work, long long work_bytes, int* status, cudaStream_t st) {
   using namespace smc;
   if (n_rows <= 0) return 0;
   if (n_rows > EV_ENTRIES || kept == nullptr || heads < 1 || keep < 1 || first < 0 || last < 0 || first > keep || last > keep - first) return -170;
-  if (bt_stride < 1 || bt_stride > (long long)EV_PIECES * EV_T || mass_stride < bt_stride || (key_pos != nullptr && kp_stride < bt_stride)) return -171;
+  const int cols = pitch_cols(bt_pitch);
+  if (!pitch_fits(bt_pitch) || cols > EV_PIECES * EV_T || mass_stride < cols || (key_pos != nullptr && kp_stride < cols)) return -171;
   if (work_bytes < smc_evict_work(n_pages) || (reinterpret_cast<uintptr_t>(work) & 3)) return -172;
   EvictParams p;
   p.table = table; p.key_pos = key_pos; p.mass = mass; p.lens = lens; p.src = src; p.dst = dst; p.kept = kept;
   p.refcount = refcount; p.free_stack = free_stack; p.free_count = free_count;
   p.done = (unsigned*)work; p.dead = p.done + 1; p.old = (int*)(p.done + 64); p.bits = p.done + 64 + EV_ENTRIES;
-  p.bt_stride = bt_stride; p.kp_stride = kp_stride; p.mass_stride = mass_stride;
+  p.bt_stride = pitch_stride(bt_pitch); p.cols = cols; p.kp_stride = kp_stride; p.mass_stride = mass_stride;
   p.n_rows = n_rows; p.rows = rows; p.heads = heads; p.n_pages = n_pages; p.keep = keep; p.first = first; p.last = last; p.status = status;
-  const long long per = (bt_stride + EV_CL * EV_T - 1) / (EV_CL * EV_T) * EV_T, alone = (bt_stride < EV_SOLO ? (bt_stride + EV_T - 1) / EV_T * EV_T : EV_SOLO);
-  p.capacity = (int)(per > alone ? per : alone);
+  const int per = (cols + EV_CL * EV_T - 1) / (EV_CL * EV_T) * EV_T, alone = cols < EV_SOLO ? (cols + EV_T - 1) / EV_T * EV_T : EV_SOLO;
+  p.capacity = per > alone ? per : alone;
   const size_t smem = (size_t)p.capacity * 4;
   CUDA_CHECK_RET(cudaFuncSetAttribute(evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchAttribute attr[1];

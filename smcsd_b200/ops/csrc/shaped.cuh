@@ -20,10 +20,15 @@ struct ShapedCache {
   const int* key_pos;            // [bt_rows, kp_stride] its position, ascending, or null
   const int2* bounds;            // per query token: first and last visible position, or null: all up to its own
   const float* slopes;           // per query head, or null
-  int bt_stride, bt_rows, kp_stride, n_pages;
+  int bt_stride, bt_cols, bt_rows, kp_stride, n_pages;                // (a table may be some columns of a wider one)
   float mul;                     // scale log2(e)
   float cap_in, cap_out;         // scale / cap and cap log2(e), 0: no cap
 };
+
+// The pitch of a block table: from row to row in the low 32 bits, its columns in the high ones (0: as many).
+inline long long pitch_stride(long long pitch) { return pitch & 0xffffffffll; }
+inline int pitch_cols(long long pitch) { return (int)(pitch >> 32 ? pitch >> 32 : pitch); }
+inline bool pitch_fits(long long pitch) { return pitch > 0 && pitch_stride(pitch) <= 0x7fffffff && pitch_cols(pitch) <= pitch_stride(pitch); }
 
 // Scales and caps (0: none) whose factors are fp32 numbers: scale log2(e), scale / cap and cap log2(e).
 inline bool shaped_scores_fit(float scale, float cap) {
@@ -32,10 +37,10 @@ inline bool shaped_scores_fit(float scale, float cap) {
 }
 
 // (in double precision: an error of a factor is one of every score)
-inline ShapedCache shaped_cache(const int* block_table, int bt_stride, int bt_rows, int n_pages, const int* key_pos, int kp_stride, const int* bounds,
+inline ShapedCache shaped_cache(const int* block_table, long long bt_pitch, int bt_rows, int n_pages, const int* key_pos, int kp_stride, const int* bounds,
                                 const float* slopes, float scale, float cap) {
   const double log2e = 1.4426950408889634;
-  return ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, bt_stride, bt_rows, kp_stride, n_pages, (float)(scale * log2e),
+  return ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, (int)pitch_stride(bt_pitch), pitch_cols(bt_pitch), bt_rows, kp_stride, n_pages, (float)(scale * log2e),
                      cap > 0.f ? (float)((double)scale / cap) : 0.f, cap > 0.f ? (float)(cap * log2e) : 0.f};
 }
 
@@ -47,7 +52,7 @@ __device__ __forceinline__ ShapedRun shaped_run(const ShapedCache& c, const int4
   const int4 v = runs[s];
   ShapedRun r{v.x, v.y, v.z, v.w};
   if (r.n <= 0) { r.n = 0; return r; }
-  if (r.row < 0 || r.row >= c.bt_rows || r.held < 0 || r.at < 0 || r.at > T - r.n || r.held > c.bt_stride - r.n) {
+  if (r.row < 0 || r.row >= c.bt_rows || r.held < 0 || r.at < 0 || r.at > T - r.n || r.held > c.bt_cols - r.n) {
     atomicOr(status, SMC_ERR_BOUNDS);
     r.n = 0;
   }

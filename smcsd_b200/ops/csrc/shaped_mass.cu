@@ -464,7 +464,7 @@ static int launch_shaped_mass(const ShapedMassParams& p, cudaStream_t st) {
 }  // namespace smc
 
 // q [T] rows of Hq * D bf16 values with their lse [T, Hq]; runs as in smc_shaped_prompt, every row once; mass [bt_rows, Hkv, mass_stride] fp32.
-SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, int n_pages, const int* block_table, int bt_stride, int bt_rows,
+SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, int n_pages, const int* block_table, long long bt_pitch, int bt_rows,
                             const int* key_pos, int kp_stride, const int* runs, int n_runs, const float* lse, float* mass, long long mass_stride,
                             int T, int Hq, int Hkv, int D, float scale, float cap, const float* slopes, const int* bounds, int* status, int pdl,
                             cudaStream_t st) {
@@ -475,9 +475,9 @@ SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, i
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -161;
   if (!shaped_scores_fit(scale, cap)) return -162;
-  if (mass_stride < bt_stride) return -163;
+  if (!pitch_fits(bt_pitch) || mass_stride < pitch_cols(bt_pitch)) return -163;
   ShapedMassParams p;
-  p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
+  p.c = shaped_cache(block_table, bt_pitch, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.runs = (const int4*)runs; p.lse = lse; p.mass = mass;
   p.ld_q = ld_q; p.mass_stride = mass_stride; p.n_runs = n_runs; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.pdl = pdl; p.status = status;
   // Two blocks to a key tile where sequences bring 16 steps and more: the first tile of a sequence, which all its tokens see, is half as long then.  4096 tokens, 32 heads of

@@ -112,7 +112,7 @@ __device__ __forceinline__ bool sp_find_tile(const ShapedCache& c, const int4* r
     return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
   };
   if (count(1) <= want) return false;
-  int lo = 1, hi = c.bt_stride / bk + 2;                              // count(lo) > want >= count(hi)
+  int lo = 1, hi = c.bt_cols / bk + 2;                                // count(lo) > want >= count(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (count(mid) > want) lo = mid; else hi = mid;
@@ -646,7 +646,7 @@ static int launch_shaped_prompt(const ShapedPromptParams& p, int n_tiles, const 
 // q, out: T rows of Hq * D bf16 values; runs [n_runs][4] int32 {block-table row, tokens held, index of the first new token in q, new tokens}:
 // all tokens of a sequence, the new ones included, are in the pages of its row.  bounds [T][2], slopes [Hq], key_pos, lse [T, Hq] may be null.
 SMC_API int smc_shaped_prompt(const void* q, long long ld_q, const void* k_pool, const void* v_pool, int n_pages, const int* block_table,
-                              int bt_stride, int bt_rows, const int* key_pos, int kp_stride, const int* runs, int n_runs, void* out,
+                              long long bt_pitch, int bt_rows, const int* key_pos, int kp_stride, const int* runs, int n_runs, void* out,
                               long long ld_out, float* lse, int T, int Hq, int Hkv, int D, float scale, float cap, const float* slopes,
                               const int* bounds, int* status, int pdl, cudaStream_t st) {
   using namespace smc;
@@ -656,10 +656,10 @@ SMC_API int smc_shaped_prompt(const void* q, long long ld_q, const void* k_pool,
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(runs) | reinterpret_cast<uintptr_t>(k_pool) |
        reinterpret_cast<uintptr_t>(v_pool)) & 15)
     return -141;
-  if ((ld_q & 7) || (ld_out & 7) || (reinterpret_cast<uintptr_t>(bounds) & 7)) return -142;
+  if (!pitch_fits(bt_pitch) || (ld_q & 7) || (ld_out & 7) || (reinterpret_cast<uintptr_t>(bounds) & 7)) return -142;
   if (!shaped_scores_fit(scale, cap)) return -143;
   ShapedPromptParams p;
-  p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
+  p.c = shaped_cache(block_table, bt_pitch, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.v_pool = (const __nv_bfloat16*)v_pool;
   p.runs = (const int4*)runs; p.out = (__nv_bfloat16*)out; p.lse = lse; p.ld_q = ld_q; p.ld_out = ld_out;
   p.n_runs = n_runs; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.pdl = pdl; p.status = status;

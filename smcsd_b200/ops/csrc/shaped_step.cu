@@ -61,7 +61,7 @@ __device__ __forceinline__ StepKeys step_keys(const ShapedStepParams& p, int s) 
   StepKeys k;
   k.row = p.rows[s];
   k.len = p.lens[s];
-  if (k.row < 0 || k.row >= p.c.bt_rows || k.len < 0 || k.len > p.c.bt_stride) {
+  if (k.row < 0 || k.row >= p.c.bt_rows || k.len < 0 || k.len > p.c.bt_cols) {
     atomicOr(p.status, SMC_ERR_BOUNDS);
     k.row = k.len = 0;
   }
@@ -764,7 +764,7 @@ SMC_API long long smc_shaped_step_work(int bs, int E, int Hq, int Hkv, int D, lo
 // q, out: bs * E rows of Hq * D bf16 values, the E tokens of a sequence are the last of its lens[s] cached ones (rows [bs], lens [bs] int32).
 // work: zeros at first, smc_shaped_step_work bytes or more; with the mass it has to hold the scores of all cached tokens of the batch.  mass [bt_rows, Hkv, mass_stride] fp32 or null.
 SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, const void* v_pool, int n_pages, const int* block_table,
-                            int bt_stride, int bt_rows, const int* key_pos, int kp_stride, const int* rows, const int* lens, void* out,
+                            long long bt_pitch, int bt_rows, const int* key_pos, int kp_stride, const int* rows, const int* lens, void* out,
                             long long ld_out, float* lse, float* mass, long long mass_stride, int bs, int E, int Hq, int Hkv, int D,
                             float scale, float cap, const float* slopes, const int* bounds, void* work, long long work_bytes,
                             int* status, int pdl, cudaStream_t st) {
@@ -776,12 +776,12 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -151;
   if (!shaped_scores_fit(scale, cap)) return -152;
-  if (mass != nullptr && mass_stride < bt_stride) return -153;
+  if (!pitch_fits(bt_pitch) || (mass != nullptr && mass_stride < pitch_cols(bt_pitch))) return -153;
   StepWork w = step_work(bs, E, Hq, Hkv, D, 0);
   if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hkv * ((E * (Hq / Hkv) + 3) / 4 * 4) * step_tile(D) * 4);       // the rest of it
   if (work_bytes < (long long)w.bytes || (mass != nullptr && w.score_tiles < 1)) return -154;
   ShapedStepParams p;
-  p.c = shaped_cache(block_table, bt_stride, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
+  p.c = shaped_cache(block_table, bt_pitch, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.v_pool = (const __nv_bfloat16*)v_pool;
   p.rows = rows; p.lens = lens; p.out = (__nv_bfloat16*)out; p.lse = lse; p.mass = mass;
   char* base = (char*)work;

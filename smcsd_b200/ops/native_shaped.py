@@ -36,9 +36,9 @@ def _library():
     global _lib
     if _lib is None:
         L, vp, i, ll, f = K.lib(), C.c_void_p, C.c_int, C.c_longlong, C.c_float
-        L.smc_shaped_prompt.argtypes = [vp, ll, vp, vp, i, vp, i, i, vp, i, vp, i, vp, ll, vp, i, i, i, i, f, f, vp, vp, vp, i, vp]
-        L.smc_shaped_step.argtypes = [vp, ll, vp, vp, i, vp, i, i, vp, i, vp, vp, vp, ll, vp, vp, ll, i, i, i, i, i, f, f, vp, vp, vp, ll, vp, i, vp]
-        L.smc_shaped_mass.argtypes = [vp, ll, vp, i, vp, i, i, vp, i, vp, i, vp, vp, ll, i, i, i, i, f, f, vp, vp, vp, i, vp]
+        L.smc_shaped_prompt.argtypes = [vp, ll, vp, vp, i, vp, ll, i, vp, i, vp, i, vp, ll, vp, i, i, i, i, f, f, vp, vp, vp, i, vp]
+        L.smc_shaped_step.argtypes = [vp, ll, vp, vp, i, vp, ll, i, vp, i, vp, vp, vp, ll, vp, vp, ll, i, i, i, i, i, f, f, vp, vp, vp, ll, vp, i, vp]
+        L.smc_shaped_mass.argtypes = [vp, ll, vp, i, vp, ll, i, vp, i, vp, i, vp, vp, ll, i, i, i, i, f, f, vp, vp, vp, i, vp]
         L.smc_evict.argtypes = [vp, ll, vp, ll, vp, ll, vp, i, vp, vp, i, i, i, i, i, vp, vp, vp, vp, i, vp, ll, vp, vp]
         L.smc_shaped_step_work.argtypes = [i, i, i, i, i, ll]
         L.smc_evict_work.argtypes = [i]
@@ -84,12 +84,12 @@ def _pool(t: torch.Tensor, name: str, dev: int, width: int) -> int:
 
 
 def _tables(block_table: torch.Tensor, key_pos: Optional[torch.Tensor], dev: int):
-    """Address, row stride and rows of the block table, address and row stride of the positions."""
+    """Address, pitch (row stride, columns above bit 32) and rows of the block table, address and row stride of the positions."""
     shape, stride = block_table.shape, block_table.stride()
     if block_table.dtype is not _I32 or block_table.get_device() != dev or len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or stride[1] != 1 or stride[0] < shape[1] and shape[0] > 1:
         raise _wrong(block_table, "block_table", f"int32 [rows, tokens] on cuda:{dev}")
     rows, cols = shape
-    bt = (block_table.data_ptr(), stride[0] if rows > 1 else cols, rows)
+    bt = (block_table.data_ptr(), (stride[0] if rows > 1 else cols) | cols << 32, rows)
     if key_pos is None:
         return bt, (None, 0)
     stride = key_pos.stride()

@@ -17,3 +17,18 @@ def test_scales_and_caps_outside_of_fp32_are_refused_ahead_of_any_launch(scale, 
     assert L.smc_shaped_prompt(p, 512, p, p, 7, p, 8, 1, None, 0, p, 1, p, 512, None, 4, 8, 2, 64, scale, cap, None, None, p, 0, None) == -143
     assert L.smc_shaped_mass(p, 512, p, 7, p, 8, 1, None, 0, p, 1, p, p, 8, 4, 8, 2, 64, scale, cap, None, None, p, 0, None) == -162
     assert L.smc_shaped_step(p, 512, p, p, 7, p, 8, 1, None, 0, p, p, p, 512, None, None, 8, 2, 1, 8, 2, 64, scale, cap, None, None, p, 1 << 30, p, 0, None) == -152
+
+
+@needs_library
+def test_pitches_are_refused_ahead_of_any_launch():
+    """From row to row in the low 32 bits, columns above them: more columns than that, none at all, weights or positions of fewer."""
+    L, p = N._library(), 1 << 20
+
+    def calls(pitch, mass_stride=8, kp_stride=8):
+        return (L.smc_shaped_prompt(p, 512, p, p, 7, p, pitch, 1, None, 0, p, 1, p, 512, None, 4, 8, 2, 64, 0.125, 0.0, None, None, p, 0, None),
+                L.smc_shaped_mass(p, 512, p, 7, p, pitch, 1, None, 0, p, 1, p, p, mass_stride, 4, 8, 2, 64, 0.125, 0.0, None, None, p, 0, None),
+                L.smc_shaped_step(p, 512, p, p, 7, p, pitch, 1, None, 0, p, p, p, 512, None, p, mass_stride, 2, 1, 8, 2, 64, 0.125, 0.0, None, None, p, 1 << 30, p, 0, None),
+                L.smc_evict(p, pitch, p, kp_stride, p, mass_stride, p, 4, p, p, 3, 2, 8, 1, 1, p, p, p, p, 100, p, 1 << 20, p, None))
+    for pitch in (0, -8, 8 | 9 << 32, 1 << 31, 1 << 40):
+        assert calls(pitch) == (-142, -163, -153, -171), pitch
+    assert calls(64 | 8 << 32, mass_stride=7)[1:] == (-163, -153, -171) and calls(64 | 8 << 32, kp_stride=7)[3] == -171

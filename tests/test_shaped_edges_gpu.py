@@ -203,3 +203,59 @@ def test_listed_positions_are_there_when_their_keys_are(Hq, Hkv, D):
         g.replay()
         assert torch.equal(out, first)
     assert torch.equal(other, first) and int(st) == 0
+
+
+# ------------------------------------------------------------------------------- tables that are columns of wider ones
+def _allocator(pages):
+    """Every page held once; free stack and its count."""
+    return torch.ones(pages + 1, dtype=torch.int32, device=DEV), torch.zeros(pages, dtype=torch.int32, device=DEV), _int([0])
+
+
+def test_columns_of_a_wider_table():
+    """Positions and weights of as many columns as the slice: the same results as with tensors of their own, and lengths that reach into the other columns raise the status."""
+    N = _N()
+    Hq, Hkv, D, cols = 8, 2, 64, 210
+    c = Cache([200, 150], Hkv, D, seed=12, shed=True)
+    wide = torch.full((3, 400), 1, dtype=torch.int32, device=DEV)
+    wide[:, :205] = c.table
+    pos = torch.zeros(3, cols, dtype=torch.int32, device=DEV)
+    pos[:, :205] = c.key_pos
+    own = wide[:, :cols].contiguous()
+    q, results = _randn(60, Hq * D, seed=13), []
+    work = torch.zeros(N.shaped_step_work_bytes(2, 1, Hq, Hkv, D, 700), dtype=torch.uint8, device=DEV)
+    ework = torch.zeros(N.evict_work_bytes(350), dtype=torch.uint8, device=DEV)
+
+    def run(table, held, n0, lens):
+        st = _int([0])
+        m = torch.zeros(3, Hkv, cols, device=DEV)
+        out, lse, out1 = torch.zeros_like(q), torch.zeros(60, Hq, device=DEV), torch.zeros(2, Hq * D, dtype=torch.bfloat16, device=DEV)
+        kw = dict(Hq=Hq, Hkv=Hkv, D=D, scale=0.125, status=st, key_pos=pos, slopes=_slopes(Hq))
+        runs = _int([[1, held, 0, n0], [2, 130, 40, 20]])
+        states = []
+        N.attention_shaped_prompt(q, c.k, c.v, table, runs, out, T=60, lse=lse, **kw)
+        states.append(int(st.clone()))
+        st.zero_()
+        N.attention_key_mass(q, c.k, table, runs, lse, m, T=60, **kw)
+        states.append(int(st.clone()))
+        st.zero_()
+        N.attention_shaped_step(q[:2], c.k, c.v, table, _int([1, 2]), _int(lens), out1, bs=2, E=1, work=work, mass=m, **kw)
+        states.append(int(st.clone()))
+        st.zero_()
+        t, p, ln = (table if table.is_contiguous() else wide.clone()[:, :cols]), pos.clone(), _int([0] + lens)
+        t = t.clone() if table.is_contiguous() else t
+        kept, mass = torch.full((2, 90), -7, dtype=torch.int32, device=DEV), m.clone()
+        refs, stack, count = _allocator(350)
+        N.evict_tokens(t, _int([1, 2]), _int([1, 2]), ln, mass, refs, stack, count, keep=90, first=2, last=9, kept=kept, work=ework, status=st, key_pos=p)
+        states.append(int(st.clone()))
+        return states, [out, lse, out1, m, t.clone(), p, ln, kept, mass, refs, stack, count]
+
+    for table in (own, wide[:, :cols]):
+        states, got = run(table, 160, 40, [200, 150])
+        assert states == [0, 0, 0, 0]
+        results.append(got)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    # beyond the columns, within the pitch: that sequence is refused, the other one served
+    states, bad = run(wide[:, :cols], 180, 40, [215, 150])
+    assert states == [8, 8, 8, 8]
+    assert not bool(bad[0][:40].any()) and not bool(bad[2][0].any()) and torch.equal(bad[0][40:], results[0][0][40:]) and torch.equal(bad[2][1], results[0][2][1])
+    assert not bool(bad[3][1].any()) and bad[6].tolist() == [0, 215, 90]
