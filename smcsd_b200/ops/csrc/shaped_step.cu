@@ -53,37 +53,83 @@ struct ShapedStepParams {
   int* status;
 };
 
-// Run of keys [begin, begin + n) of a sequence that any of its tokens may see; with listed positions an outer bound of it: positions are
-// distinct, so tokens lie at least as far apart in position as in the row.
+// Run of keys [begin, begin + n) of a sequence between the first and the last one that any of its tokens sees.
 struct StepKeys { int row, len, begin, n; };
 
-__device__ __forceinline__ StepKeys step_keys(const ShapedStepParams& p, int s) {
-  StepKeys k;
-  k.row = p.rows[s];
-  k.len = p.lens[s];
-  if (k.row < 0 || k.row >= p.c.bt_rows || k.len < 0 || k.len > p.c.bt_cols) {
-    atomicOr(p.status, SMC_ERR_BOUNDS);
-    k.row = k.len = 0;
-  }
-  int lo = 0, hi = k.len;
-  if (p.c.bounds != nullptr) {
-    lo = k.len;
-    hi = 0;
-    for (int e = 0; e < p.E; ++e) {
-      const int idx = k.len - p.E + e;
-      if (idx < 0) continue;
-      const int pos = p.c.key_pos != nullptr ? p.c.key_pos[(size_t)k.row * p.c.kp_stride + idx] : idx;
-      const int2 b = shaped_bounds(p.c, s * p.E + e, pos);
-      if (b.x > b.y) continue;
-      lo = min(lo, p.c.key_pos == nullptr ? b.x : max(0, b.x <= pos ? idx - (pos - b.x) : idx));
-      hi = max(hi, p.c.key_pos == nullptr ? b.y + 1 : b.y >= pos ? idx + 1 + min(b.y - pos, k.len) : min(idx, b.y + 1));
+// What the schedule leaves in shared memory: tiles of the sequences ahead of each, [bs + 1], and where its run begins with the keys of its last tile less one, [bs].
+struct StepLine { int* tiles; int* spans; };
+constexpr int ST_LAST_BITS = 7;                        // keys of a tile: at most 128; a run begins in front of 2^24
+
+// of a sequence that has a tile
+__device__ __forceinline__ StepKeys step_keys(const ShapedStepParams& p, const StepLine& line, int s) {
+  const int span = line.spans[s];
+  return {p.rows[s], p.lens[s], span >> ST_LAST_BITS, (line.tiles[s + 1] - line.tiles[s] - 1) * p.tile + (span & ((1 << ST_LAST_BITS) - 1)) + 1};
+}
+
+// The runs of all sequences, each found by L lanes of a warp: tiles into line.tiles[s + 1], beginnings into line.spans[s].  Listed positions are searched for the ends of the
+// intervals, L probes at a time, inside what their distances leave: positions are distinct, so tokens lie at least as far apart in position as in the row.
+template <int L, bool SEARCH>
+__device__ __forceinline__ void step_spans(const ShapedStepParams& p, const StepLine& line) {
+  const int lane = threadIdx.x & 31, sub = lane % L, shift = lane / L * L;
+  const unsigned group = L == 32 ? 0xffffffffu : (1u << L) - 1u;
+  for (int s0 = 0; s0 < p.bs; s0 += (int)blockDim.x / L) {
+    const int s = s0 + (int)threadIdx.x / L;
+    int row = 0, len = 0;
+    if (s < p.bs) {
+      row = p.rows[s];
+      len = p.lens[s];
+      if (row < 0 || row >= p.c.bt_rows || len < 0 || len > min(p.c.bt_cols, SH_POS_END)) {
+        atomicOr(p.status, SMC_ERR_BOUNDS);
+        row = len = 0;
+      }
     }
-    lo = min(lo, k.len);
-    hi = min(hi, k.len);
+    int lo = 0, hi = len;
+    if (p.c.bounds != nullptr) {
+      const int* kp = p.c.key_pos != nullptr ? p.c.key_pos + (size_t)row * p.c.kp_stride : nullptr;
+      int near = SH_POS_END, far = -1;                 // positions that any token sees
+      lo = len;
+      hi = 0;
+      for (int e = sub; e < p.E; e += L) {
+        const int idx = len - p.E + e;
+        if (idx < 0) continue;
+        const int pos = kp != nullptr ? kp[idx] : idx;
+        const int2 b = shaped_bounds(p.c, s * p.E + e, pos);
+        if (b.x > b.y) continue;
+        near = min(near, b.x);
+        far = max(far, b.y);
+        lo = min(lo, kp == nullptr ? b.x : max(0, b.x <= pos ? idx - (pos - b.x) : idx));
+        hi = max(hi, kp == nullptr ? b.y + 1 : b.y >= pos ? idx + 1 + min(b.y - pos, len) : min(idx, b.y + 1));
+      }
+#pragma unroll
+      for (int o = 1; o < L; o <<= 1) {
+        lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        near = min(near, __shfl_xor_sync(0xffffffffu, near, o));
+        far = max(far, __shfl_xor_sync(0xffffffffu, far, o));
+      }
+      lo = min(lo, len);
+      hi = max(lo, min(hi, len));
+      if constexpr (SEARCH) {
+        // first indices of [lo, hi) whose positions are >= near and > far; hi if none
+        int a0 = lo, a1 = hi, b0 = lo, b1 = hi;
+        while (__any_sync(0xffffffffu, a0 < a1 || b0 < b1)) {
+          const int sa = (a1 - a0) / (L + 1) + 1, sb = (b1 - b0) / (L + 1) + 1, at = a0 + (sub + 1) * sa - 1, bt = b0 + (sub + 1) * sb - 1;
+          const int ka = __popc(__ballot_sync(0xffffffffu, at < a1 && kp[at] < near) >> shift & group);
+          const int kb = __popc(__ballot_sync(0xffffffffu, bt < b1 && kp[bt] <= far) >> shift & group);
+          a1 = min(a1, a0 + (ka + 1) * sa - 1);
+          b1 = min(b1, b0 + (kb + 1) * sb - 1);
+          a0 += ka * sa;
+          b0 += kb * sb;
+        }
+        lo = a0;
+        hi = max(a0, b0);
+      }
+    }
+    if (s < p.bs && sub == 0) {
+      line.tiles[s + 1] = (hi - lo + p.tile - 1) / p.tile;
+      line.spans[s] = lo << ST_LAST_BITS | ((hi - lo + p.tile - 1) % p.tile);
+    }
   }
-  k.begin = lo;
-  k.n = max(0, hi - lo);
-  return k;
 }
 
 // first tile of worker w
@@ -115,13 +161,19 @@ __device__ __forceinline__ uint32_t st_pack(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// Prefix sums of the tiles of all sequences into tiles[0 .. bs], by the whole block.
-__device__ __forceinline__ void step_schedule(const ShapedStepParams& p, int* tiles, int* warp_sum) {
+// The line of all sequences, by the whole block.  A run that has to be searched for takes as many lanes as there are: its probes are dependent reads (300 sequences of up to 500
+// tokens by eight lanes each, in seven turns, 45 us a step, by one each 38).
+__device__ __forceinline__ void step_schedule(const ShapedStepParams& p, const StepLine& line, int* warp_sum) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (p.c.bounds == nullptr || p.c.key_pos == nullptr) step_spans<1, false>(p, line);
+  else if (p.bs <= warps) step_spans<32, true>(p, line);
+  else if (p.bs <= warps * 4) step_spans<8, true>(p, line);
+  else step_spans<1, true>(p, line);
+  __syncthreads();
   int base = 0;
   for (int s0 = 0; s0 < p.bs; s0 += blockDim.x) {
     const int s = s0 + threadIdx.x;
-    int sum = s < p.bs ? (step_keys(p, s).n + p.tile - 1) / p.tile : 0;
+    int sum = s < p.bs ? line.tiles[s + 1] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, sum, o);
@@ -134,11 +186,11 @@ __device__ __forceinline__ void step_schedule(const ShapedStepParams& p, int* ti
       if (w < warp) sum += warp_sum[w];
       all += warp_sum[w];
     }
-    if (s < p.bs) tiles[s + 1] = base + sum;
+    if (s < p.bs) line.tiles[s + 1] = base + sum;
     base = all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) tiles[0] = 0;
+  if (threadIdx.x == 0) line.tiles[0] = 0;
   __syncthreads();
 }
 
@@ -165,19 +217,19 @@ struct StCfg {
   static constexpr bool BULK = D == 256;
   static constexpr int SLOTS = D == 256 ? (ROWS == 8 ? 2 : 1) : 64 / ROWS;           // states that groups leave at once when they are joined
   static constexpr size_t KV = (size_t)KT * LD * 2;                // one of K, V
-  // stages, states, positions of the tiles in flight, prefix sums
-  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)SLOTS * ROWS * (D + 4) * 4 + (size_t)STAGES * KT * 4 + (ST_MAX_BS + 1 + 64) * 4;
+  // stages, states, positions of the tiles in flight, the line of tiles
+  static constexpr size_t SMEM = STAGES * 2 * KV + (size_t)SLOTS * ROWS * (D + 4) * 4 + (size_t)STAGES * KT * 4 + (2 * ST_MAX_BS + 1 + 64) * 4;
 };
 
 // A place in the line of tiles: the sequence that tile x belongs to.
 struct StepCursor {
   int s, seq0, seq1;
   StepKeys key;
-  __device__ __forceinline__ void seek(const ShapedStepParams& p, const int* tiles, int x) {
-    s = step_sequence(tiles, p.bs, x);
-    seq0 = tiles[s];
-    seq1 = tiles[s + 1];
-    key = step_keys(p, s);
+  __device__ __forceinline__ void seek(const ShapedStepParams& p, const StepLine& line, int x) {
+    s = step_sequence(line.tiles, p.bs, x);
+    seq0 = line.tiles[s];
+    seq1 = line.tiles[s + 1];
+    key = step_keys(p, line, s);
   }
 };
 
@@ -212,7 +264,8 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
   float* join = reinterpret_cast<float*>(st_smem + STAGES * 2 * Cfg::KV);            // [slot][ROWS][D + 4]
   int* pos_s = reinterpret_cast<int*>(join + Cfg::SLOTS * Cfg::ROWS * (D + 4));      // [stage][KT]
   int* tiles = pos_s + STAGES * KT;                                  // [bs + 1]
-  int* misc = tiles + ST_MAX_BS + 1;                                 // [64]
+  const StepLine line{tiles, tiles + ST_MAX_BS + 1};
+  int* misc = line.spans + ST_MAX_BS;                                // [64]
   __shared__ float ml_s[Cfg::GROUPS][Cfg::ROWS][2];
   __shared__ float4 row_s[Cfg::ROWS];                                // of a row: first and last visible position, its own, slope
   __shared__ StShared S;
@@ -231,7 +284,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
   // a mass kernel behind this one reads rows and lengths ahead of its wait: they have to be there before it may start
   if (p.pdl) pdl_wait_prior_grid();
   pdl_launch_dependents();
-  step_schedule(p, tiles, misc);
+  step_schedule(p, line, misc);
   const int total = tiles[p.bs];
   // sequences without a tile have nobody else to write their rows
   if (w == 0) {
@@ -272,7 +325,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
       if (next >= t_end) return;
       if (next >= seq_end) {
         StepCursor cur;
-        cur.seek(p, tiles, next);
+        cur.seek(p, line, next);
         seq_end = cur.seq1;
         n = cur.key.n;
         i = (next - cur.seq0) * KT + kl0;
@@ -343,7 +396,7 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
   while (x < t_end) {
     // ---------------------------------------------------------------- one sequence's tiles of this worker
     const int s = step_sequence(tiles, p.bs, x), seq0 = tiles[s], seq1 = tiles[s + 1], x_end = min(t_end, seq1);
-    const StepKeys key = step_keys(p, s);
+    const StepKeys key = step_keys(p, line, s);
     for (int r = threadIdx.x; r < Cfg::ROWS; r += THREADS) {
       const int idx = key.len - p.E + r / G;
       float4 v = make_float4((float)SH_POS_END, -1.f, 0.f, 0.f);
@@ -649,10 +702,11 @@ __global__ void __launch_bounds__(StCfg<D, NQ, MT>::THREADS, 1) shaped_step_kern
 constexpr int SM_WARPS = 8;
 
 __global__ void __launch_bounds__(SM_WARPS * 32) shaped_step_mass_kernel(const ShapedStepParams p) {
-  extern __shared__ int sm_tiles[];                                  // [bs + 1 + 32]
+  extern __shared__ int sm_tiles[];                                  // [bs + 1], [bs], [32]
   __shared__ __align__(16) float top_s[SM_WARPS][64];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y, G = p.Hq / p.Hkv, M = p.E * G, pitch = (M + 3) / 4 * 4;
-  step_schedule(p, sm_tiles, sm_tiles + p.bs + 1);                   // from what was there before the first kernel
+  const StepLine line{sm_tiles, sm_tiles + p.bs + 1};
+  step_schedule(p, line, line.spans + p.bs);                         // from what was there before the first kernel
   const int total = sm_tiles[p.bs], many = gridDim.x * SM_WARPS, me = blockIdx.x * SM_WARPS + warp;
   // on every path: whoever follows waits for this grid alone, which must not end ahead of the first kernel
   pdl_wait_prior_grid();
@@ -664,7 +718,7 @@ __global__ void __launch_bounds__(SM_WARPS * 32) shaped_step_mass_kernel(const S
   int x = step_first(me, many, total);
   while (x < x_end) {
     StepCursor cur;
-    cur.seek(p, sm_tiles, x);
+    cur.seek(p, line, x);
     const int end = min(x_end, cur.seq1);
     bool twice = false;                                              // a row listed twice would be added to by two warps at once
     for (int o = lane; o < cur.s; o += 32) twice |= p.rows[o] == cur.key.row && p.lens[o] > 0;
@@ -746,7 +800,7 @@ static int launch_shaped_step(const ShapedStepParams& p, cudaStream_t st) {
   if (p.mass == nullptr) return 0;
   cfg.gridDim = dim3((unsigned)((148 * 4 + p.Hkv - 1) / p.Hkv), (unsigned)p.Hkv);
   cfg.blockDim = dim3(SM_WARPS * 32);
-  cfg.dynamicSmemBytes = (size_t)(p.bs + 1 + 32) * 4;
+  cfg.dynamicSmemBytes = (size_t)(2 * p.bs + 1 + 32) * 4;
   cfg.numAttrs = 1;
   CUDA_CHECK_RET(cudaLaunchKernelEx(&cfg, shaped_step_mass_kernel, p));
   return 0;

@@ -259,3 +259,43 @@ def test_columns_of_a_wider_table():
     assert states == [8, 8, 8, 8]
     assert not bool(bad[0][:40].any()) and not bool(bad[2][0].any()) and torch.equal(bad[0][40:], results[0][0][40:]) and torch.equal(bad[2][1], results[0][2][1])
     assert not bool(bad[3][1].any()) and bad[6].tolist() == [0, 215, 90]
+
+
+# ------------------------------------------------------------------------------- what no token sees
+@pytest.mark.parametrize("Hq,Hkv,D,E", [(32, 8, 64, 1), (16, 4, 128, 1), (16, 4, 128, 5), (16, 2, 256, 1), (16, 2, 256, 2)])
+@pytest.mark.parametrize("shed", [False, True])
+@pytest.mark.parametrize("copies", [1, 6, 12])
+def test_step_reads_nothing_outside_of_the_intervals(Hq, Hkv, D, E, shed, copies):
+    """Keys and values that no token of their sequence sees are NaN: a window's, a document's, those ahead of where a mask ends, all of a sequence whose masks are empty."""
+    N = _N()
+    lens = [900, 300, 64, 1, 2000, 517, 130] * copies
+    bs = len(lens)
+    c = Cache(lens, Hkv, D, seed=D + E, shed=shed)
+    runs = [(i + 1, n - E, i * E, E) for i, n in enumerate(lens)]
+    b = torch.zeros(bs * E, 2, dtype=torch.int32, device=DEV)
+    for i, n in enumerate(lens):
+        pos = c.positions(i + 1)
+        own = torch.cat([torch.full((max(0, E - n),), -1, device=DEV), pos[max(n - E, 0):]])
+        last = int(pos[-1])
+        b[i * E:(i + 1) * E] = (N.score_bounds(own, window=100), N.score_bounds(own, doc_first=own.clamp(min=0) // 290 * 290), _int([[last // 4, last // 2]] * E),
+                                N.score_bounds(own), _int([[9, 8]] * E), _int([[0, last // 3]] * E), _int([[last + 1, last + 50]] * E))[i % 7]
+        see = b[i * E + max(0, E - n):(i + 1) * E]
+        see = see[see[:, 0] <= see[:, 1]]
+        unseen = (pos < see[:, 0].min()) | (pos > see[:, 1].max()) if len(see) else torch.ones_like(pos, dtype=torch.bool)
+        hidden = c.table[i + 1, :n][unseen].long()
+        c.k[hidden] = c.v[hidden] = float("nan")
+    q, st = _randn(bs * E, Hq * D, seed=14), _int([0])
+    clean = Cache(lens, Hkv, D, seed=D + E, shed=shed)
+    want, want_lse, mass = attend(clean, runs, q, Hq, scale=D ** -0.5, softcap=20.0, bounds=b)
+    out, lse, m = torch.zeros_like(q), torch.zeros(bs * E, Hq, device=DEV), torch.zeros(bs + 1, Hkv, c.table.shape[1], device=DEV)
+    work = torch.zeros(N.shaped_step_work_bytes(bs, E, Hq, Hkv, D, sum(lens)), dtype=torch.uint8, device=DEV)
+    N.attention_shaped_step(q, c.k, c.v, c.table, torch.arange(1, bs + 1, device=DEV).int(), _int(lens), out, bs=bs, E=E, Hq=Hq, Hkv=Hkv, D=D, scale=D ** -0.5, softcap=20.0,
+                            status=st, work=work, bounds=b, key_pos=c.key_pos, lse=lse, mass=m)
+    torch.cuda.synchronize()
+    assert int(st) == 0
+    moved = _score_error(clean, q, D ** -0.5) + 3e-6 * 20 + 2.0 ** -20
+    assert float((out.double().view(want.shape) - want).abs().max()) <= _out_error(clean, moved)
+    there = torch.isfinite(want_lse)
+    assert torch.equal(torch.isfinite(lse), there) and float((lse.double() - want_lse)[there].abs().max()) <= moved
+    for row, w in mass.items():
+        assert bool(((m[row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
