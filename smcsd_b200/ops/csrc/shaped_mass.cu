@@ -20,6 +20,10 @@
 namespace smc {
 
 constexpr int MS_LOADERS = 4, MS_Q = 128;
+// A sequence that brings so many steps and has no more key tiles, over all heads, than the device has SMs: two blocks share each of them.  Its own numbers decide, so that
+// the order of its sums does not hang on what else a call brings.  Heads of 128, 8 KV heads, capped, us with one block and with two: 1500 tokens (48 tiles) 155 and 84, 4096
+// (128) 356 and 195, 9000 (288) 759 and 772, two of 400 behind 6000 (208 each) 131 and 161: a tile costs 8 us before its first sum in every block.
+constexpr int MS_SHARED_STEPS = 16, MS_SHARED_TILES = 148;
 
 template <int D> struct MsCfg;                        // key tiles of a CTA, slots of the ring of query steps, of them in flight, sets of keys in shared memory
 template <> struct MsCfg<64> { static constexpr int NT = 2, QU = 6, LAG = 3, KB = 2; };
@@ -34,7 +38,7 @@ struct ShapedMassParams {
   const float* lse;              // [T, Hq]
   float* mass;                   // [bt_rows, Hkv, mass_stride]
   long long ld_q, mass_stride;
-  int n_runs, T, Hq, Hkv, pdl, cluster;
+  int n_runs, T, Hq, Hkv, pdl, cluster, share_from;                  // blocks of a cluster; new tokens of a sequence whose tiles two of them share
   int* status;
 };
 
@@ -70,13 +74,20 @@ __device__ __forceinline__ bool ms_wait(Shared& S, int* status, uint64_t* bar, u
   }
 }
 
-// All tiles of KT keys of all sequences, those with most tokens behind their first key in front; used by whole warps.
+// All tiles of KT keys of the sequences whose tiles two blocks share, or of the others, those with most tokens behind their first key in front; used by whole warps.
 template <int KT>
 struct MsTiles {
   const ShapedMassParams& p;
+  const bool shared;
   ShapedRun mine;
-  __device__ explicit MsTiles(const ShapedMassParams& params) : p(params) { mine = run_of((int)threadIdx.x & 31); }
-  __device__ ShapedRun run_of(int s) const { return s < p.n_runs ? shaped_run(p.c, p.runs, s, p.T, p.status) : ShapedRun{0, 0, 0, 0}; }
+  __device__ MsTiles(const ShapedMassParams& params, const ShapedRun& of_lane, bool of_shared) : p(params), shared(of_shared), mine(this_kind(of_lane)) {}
+  __device__ static ShapedRun any_run(const ShapedMassParams& p, int s) { return s < p.n_runs ? shaped_run(p.c, p.runs, s, p.T, p.status) : ShapedRun{0, 0, 0, 0}; }
+  __device__ ShapedRun this_kind(ShapedRun r) const {
+    const bool is_shared = p.cluster > 1 && r.n >= p.share_from && (long long)((r.held + r.n - 1) / KT + 1) * p.Hkv <= MS_SHARED_TILES;
+    if (is_shared != shared) r.n = 0;
+    return r;
+  }
+  __device__ ShapedRun run_of(int s) const { return this_kind(any_run(p, s)); }
   // tiles of run r with at least `tokens` of its new tokens at or behind their first key: the first ones of the row
   __device__ int of_run(const ShapedRun& r, int tokens) const { return tokens > r.n ? 0 : (int)((unsigned)(r.held + r.n - tokens) / KT) + 1; }
   __device__ int count(int tokens) const {
@@ -87,7 +98,9 @@ struct MsTiles {
   // tile number `want`: its run, the run's number and the tile inside it
   __device__ bool find(int want, ShapedRun& run, int& number, int& tile) const {
     const int lane = threadIdx.x & 31;
-    int lo = 1, hi = p.T + 1;                         // count(lo) > want >= count(hi)
+    int most = mine.n;
+    for (int s = lane + 32; s < p.n_runs; s += 32) most = max(most, run_of(s).n);
+    int lo = 1, hi = __reduce_max_sync(0xffffffffu, most) + 1;        // count(lo) > want >= count(hi)
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (count(mid) > want) lo = mid; else hi = mid;
@@ -161,17 +174,21 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
   const uint32_t tmem_base = S.tmem_slot;
   if (p.pdl) { pdl_launch_dependents(); pdl_wait_prior_grid(); }
 
-  const MsTiles<NT * 128> all(p);
-  const int items = all.count(1) * p.Hkv;             // (at most the table's entries over 128, times the heads)
   bool dead = false;                                  // a wait of this warp ran out: it goes on to the end without work
   uint32_t u0 = 0, k_use = 0;                         // steps and key tiles so far: barriers run on from item to item
-  const int C = p.cluster, rank = C > 1 ? (int)cluster_ctarank() : 0, groups = gridDim.x / C, group = blockIdx.x / C;
-  for (int base = 0, round = 0; base < items; base += groups, ++round) {
+  using Tiles = MsTiles<NT * 128>;
+  const ShapedRun of_lane = Tiles::any_run(p, lane);
+  // tiles that two blocks share, then the others (at most the table's entries over 128, times the heads)
+  const int together = p.cluster > 1 ? Tiles(p, of_lane, true).count(1) * p.Hkv : 0, items = together + Tiles(p, of_lane, false).count(1) * p.Hkv;
+  for (int base = 0, round = 0; base < items; ++round) {
+    const bool shared = base < together;
+    const int C = shared ? p.cluster : 1, rank = C > 1 ? (int)cluster_ctarank() : 0, groups = gridDim.x / C, group = blockIdx.x / C;
     // every second round runs backwards, so that who had a long tile gets a short one
-    const int item = base + (round & 1 ? groups - 1 - group : group);
+    const int item = base + (round & 1 ? groups - 1 - group : group), end = shared ? together : items, first = shared ? 0 : together;
+    base = min(base + groups, end);
     ShapedRun run{0, 0, 0, 0};
     int number = 0, tile = 0;
-    bool have = item < items && all.find(item / p.Hkv, run, number, tile);
+    bool have = item < end && Tiles(p, of_lane, shared).find((item - first) / p.Hkv, run, number, tile);
     if (have) {
       bool twice = false;                             // a row listed twice would be added to by two blocks at once
       for (int o = lane; o < number; o += 32) twice |= p.runs[o].x == run.row && p.runs[o].w > 0;
@@ -444,7 +461,7 @@ static int launch_shaped_mass(const ShapedMassParams& p, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   // as many clusters as the device holds at once (fewer than its SMs would make: a cluster stays inside a GPC), looked up once for each device
-  static std::atomic<int> held[64][9];
+  static std::atomic<int> held[64][3];
   int dev = 0;
   CUDA_CHECK_RET(cudaGetDevice(&dev));
   int clusters = dev < 64 ? held[dev][p.cluster].load(std::memory_order_relaxed) : 0;
@@ -480,10 +497,8 @@ SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, i
   p.c = shaped_cache(block_table, bt_pitch, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.runs = (const int4*)runs; p.lse = lse; p.mass = mass;
   p.ld_q = ld_q; p.mass_stride = mass_stride; p.n_runs = n_runs; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.pdl = pdl; p.status = status;
-  // Two blocks to a key tile where sequences bring 16 steps and more: the first tile of a sequence, which all its tokens see, is half as long then.  4096 tokens, 32 heads of
-  // 128 on 8: one block 318 us, two 200, four 240, eight 297 - a tile costs 8 us before its first sum in every block.
-  const long long steps = (long long)T / n_runs * (Hq / Hkv) / 128;
-  p.cluster = steps >= 16 ? 2 : 1;
+  p.share_from = MS_SHARED_STEPS * (128 / (Hq / Hkv));
+  p.cluster = T >= p.share_from ? 2 : 1;      // clusters only where a sequence may bring that many steps
 #define SMC_SHAPED_MASS(DD)                                                                                            \
   if (D == DD) {                                                                                                       \
     if (cap > 0.f) return slopes ? launch_shaped_mass<DD, true, true>(p, st) : launch_shaped_mass<DD, true, false>(p, st); \

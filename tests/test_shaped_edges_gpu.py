@@ -299,3 +299,54 @@ def test_step_reads_nothing_outside_of_the_intervals(Hq, Hkv, D, E, shed, copies
     assert torch.equal(torch.isfinite(lse), there) and float((lse.double() - want_lse)[there].abs().max()) <= moved
     for row, w in mass.items():
         assert bool(((m[row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
+
+
+# ------------------------------------------------------------------------------- the mass of some tokens of a pass
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (16, 4, 128), (6, 2, 128), (8, 1, 256)])
+def test_key_mass_bits_depend_on_the_sequence_alone(Hq, Hkv, D):
+    """A long sequence alone, beside many short ones, and as some runs of a longer pass: the same bits."""
+    N = _N()
+    n, got, st = 2100, [], _int([0])
+    for others in (0, 40):
+        c = Cache([n] + [3] * others, Hkv, D, seed=21, order="up")
+        c.k[1:n + 1] = _randn(n, Hkv * D, seed=22)
+        q = torch.cat([_randn(n, Hq * D, seed=23), _randn(3 * others, Hq * D, seed=24)])
+        lse = torch.full((len(q), Hq), 4.0, device=DEV)
+        runs = [[1, 0, 0, n]] + [[2 + i, 0, n + 3 * i, 3] for i in range(others)]
+        kw = dict(Hq=Hq, Hkv=Hkv, D=D, scale=D ** -0.5, status=st, softcap=30.0)
+        for listed in (runs, runs[:1], runs[::-1]):
+            m = torch.zeros(others + 2, Hkv, c.table.shape[1], device=DEV)
+            N.attention_key_mass(q, c.k, c.table, _int(listed), lse, m, T=len(q), **kw)
+            got.append(m[1, :, :n].clone())
+    torch.cuda.synchronize()
+    assert int(st) == 0 and all(torch.equal(got[0], x) for x in got[1:])
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 64), (16, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("mask", ["causal", "window", "prefix"])
+def test_key_mass_of_the_last_tokens_of_a_pass(Hq, Hkv, D, mask):
+    """``runs`` lists the last tokens of each prompt of a pass: their mass alone, and the bits of a call that is handed those tokens only."""
+    N = _N()
+    sizes, tail = [3000, 40, 900], [64, 40, 33]
+    c = Cache(sizes, Hkv, D, seed=25, shed=True)
+    T, starts = sum(sizes), [0, 3000, 3040]
+    q, st, scale = _randn(T, Hq * D, seed=26), _int([0]), D ** -0.5
+    pos = torch.cat([c.positions(i + 1) for i in range(3)])
+    b = {"causal": None, "window": N.score_bounds(pos, window=500), "prefix": N.score_bounds(pos, prefix=300)}[mask]
+    tails = [(i + 1, n - k, at + n - k, k) for i, (n, k, at) in enumerate(zip(sizes, tail, starts))]
+    kw = dict(Hq=Hq, Hkv=Hkv, D=D, scale=scale, status=st, key_pos=c.key_pos, softcap=30.0, slopes=_slopes(Hq))
+    _, want_lse, mass = attend(c, tails, q, Hq, scale=scale, softcap=30.0, slopes=_slopes(Hq), bounds=b)
+    lse = want_lse.float()
+    m = [torch.zeros(4, Hkv, c.table.shape[1], device=DEV) for _ in range(2)]
+    N.attention_key_mass(q, c.k, c.table, _int(tails), lse, m[0], T=T, bounds=b, **kw)
+    take = torch.cat([torch.arange(at, at + k, device=DEV) for _, _, at, k in tails])
+    alone, at = [], 0
+    for row, held, _, k in tails:
+        alone.append((row, held, at, k))
+        at += k
+    N.attention_key_mass(q[take], c.k, c.table, _int(alone), lse[take], m[1], T=len(take), bounds=None if b is None else b[take].contiguous(), **kw)
+    torch.cuda.synchronize()
+    assert int(st) == 0 and torch.equal(m[0], m[1])
+    moved = _score_error(c, q, scale) + 3e-6 * 30 + 2.0 ** -20
+    for row, w in mass.items():
+        assert bool(((m[0][row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
