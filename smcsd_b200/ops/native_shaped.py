@@ -192,10 +192,14 @@ def evict_tokens(block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor
                  status: torch.Tensor, key_pos: Optional[torch.Tensor] = None) -> None:
     """Of the ``lens[row]`` tokens of each row in ``src`` [n] the first ``first``, the last ``last`` and those between with the highest sum of ``mass`` over the KV
     heads stay, at most ``keep`` in all (equal sums: the lower index).  They move, in their order, with page, position and weights to the row
-    in ``dst``: the same one, whose other tokens give up their pages' references, or another, free one, which takes references.  ``lens`` [rows]
+    in ``dst``: the same one, whose other tokens give up their pages' references, or another, free one, which takes references.  Without ``key_pos`` they are known by their
+    new indices from then on, which is right for attention without ``bounds`` and ``slopes`` only.  ``lens`` [rows]
     is updated, ``kept`` [n, keep] receives the indices (-1 behind the last).  Weights behind the kept tokens are cleared up to the old length of the row; its other
-    entries there are left as they were.  A row may be written by one entry only, and then be read by no other."""
+    entries there are left as they were.  A row may be written by one entry only, and then be read by no other.  At most 4096 entries, block tables of at most 262144 columns
+    (one of more is handed over as a slice of them)."""
     L, dev = _library(), _device(block_table)
+    if src.shape[0] > 4096 or block_table.dim() == 2 and block_table.shape[1] > 262144:
+        raise ValueError(f"at most 4096 entries and 262144 columns of a block table expected, got {src.shape[0]} and {block_table.shape[1]}")
     (bt, bts, R), (kp, kps) = _tables(block_table, key_pos, dev)
     n, heads, pages = src.shape[0], mass.shape[1], refcount.shape[0] - 1
     mp, ms = _weights(mass, dev, R, heads, block_table.shape[1])

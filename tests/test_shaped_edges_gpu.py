@@ -350,3 +350,28 @@ def test_key_mass_of_the_last_tokens_of_a_pass(Hq, Hkv, D, mask):
     moved = _score_error(c, q, scale) + 3e-6 * 30 + 2.0 ** -20
     for row, w in mass.items():
         assert bool(((m[0][row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
+
+
+# ------------------------------------------------------------------------------- eviction
+def test_evict_from_a_table_of_more_columns_than_it_takes():
+    """Refused by name; a slice of the table is served, and rows of 262,144 tokens are."""
+    N = _N()
+    n, width, st = 262144, 300000, _int([0])
+    wide = torch.arange(1, width + 1, dtype=torch.int32, device=DEV).repeat(2, 1)
+    mass = torch.rand(2, 1, width, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    refs, stack, count = _allocator(width)
+    work = torch.zeros(N.evict_work_bytes(width), dtype=torch.uint8, device=DEV)
+    lens, kept, one = _int([0, n]), torch.zeros(1, 100, dtype=torch.int32, device=DEV), _int([1])
+    args = dict(keep=100, first=4, last=10, kept=kept, work=work, status=st)
+    with pytest.raises(ValueError, match="262144"):
+        N.evict_tokens(wide, one, one, lens, mass, refs, stack, count, **args)
+    with pytest.raises(ValueError, match="4096"):
+        N.evict_tokens(wide[:, :n], one.repeat(4097), one.repeat(4097), lens, mass, refs, stack, count, **{**args, "kept": kept.repeat(4097, 1)})
+    before = mass[1, 0].clone()
+    N.evict_tokens(wide[:, :n], one, one, lens, mass, refs, stack, count, **args)
+    torch.cuda.synchronize()
+    inner = before[4:n - 10].sort(descending=True, stable=True).indices[:86].sort().values + 4
+    want = torch.cat([torch.arange(4, device=DEV), inner, torch.arange(n - 10, n, device=DEV)])
+    assert int(st) == 0 and lens.tolist() == [0, 100] and int(count) == n - 100
+    assert torch.equal(kept[0].long(), want) and torch.equal(wide[1, :100].long(), want + 1) and torch.equal(mass[1, 0, :100], before[want])
+    assert not bool(mass[1, 0, 100:n].any()) and torch.equal(mass[1, 0, n:], before[n:])
