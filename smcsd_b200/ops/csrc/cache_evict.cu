@@ -291,8 +291,8 @@ __global__ void __launch_bounds__(EV_T, 2) evict_kernel(const EvictParams p) {
     while (w != 0u) {
       const int bit = 31 - __clz(w);
       w ^= 1u << bit;
-      if (put < p.n_pages) p.free_stack[put] = (top - i) * 32 + bit;
-      else atomicOr(p.status, SMC_ERR_BOUNDS);         // more free pages than there are
+      if (put >= 0 && put < p.n_pages) p.free_stack[put] = (top - i) * 32 + bit;
+      else atomicOr(p.status, SMC_ERR_BOUNDS);         // a count below zero, or more free pages than there are
       ++put;
     }
   }
@@ -370,7 +370,7 @@ SMC_API int smc_evict(int* table, long long bt_pitch, int* key_pos, long long kp
   if (n_rows > EV_ENTRIES || kept == nullptr || heads < 1 || keep < 1 || first < 0 || last < 0 || first > keep || last > keep - first) return -170;
   const int cols = pitch_cols(bt_pitch);
   if (!pitch_fits(bt_pitch) || cols > EV_PIECES * EV_T || mass_stride < cols || (key_pos != nullptr && kp_stride < cols)) return -171;
-  if (work_bytes < smc_evict_work(n_pages) || (reinterpret_cast<uintptr_t>(work) & 3)) return -172;
+  if (n_pages < 1 || work_bytes < smc_evict_work(n_pages) || (reinterpret_cast<uintptr_t>(work) & 3)) return -172;
   EvictParams p;
   p.table = table; p.key_pos = key_pos; p.mass = mass; p.lens = lens; p.src = src; p.dst = dst; p.kept = kept;
   p.refcount = refcount; p.free_stack = free_stack; p.free_count = free_count;

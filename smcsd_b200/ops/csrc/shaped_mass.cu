@@ -492,7 +492,7 @@ SMC_API int smc_shaped_mass(const void* q, long long ld_q, const void* k_pool, i
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -161;
   if (!shaped_scores_fit(scale, cap)) return -162;
-  if (!pitch_fits(bt_pitch) || mass_stride < pitch_cols(bt_pitch)) return -163;
+  if (!pitch_fits(bt_pitch) || n_pages < 0 || mass_stride < pitch_cols(bt_pitch)) return -163;
   ShapedMassParams p;
   p.c = shaped_cache(block_table, bt_pitch, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);
   p.q = (const __nv_bfloat16*)q; p.k_pool = (const __nv_bfloat16*)k_pool; p.runs = (const int4*)runs; p.lse = lse; p.mass = mass;

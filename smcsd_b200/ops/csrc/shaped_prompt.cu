@@ -656,7 +656,7 @@ SMC_API int smc_shaped_prompt(const void* q, long long ld_q, const void* k_pool,
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(runs) | reinterpret_cast<uintptr_t>(k_pool) |
        reinterpret_cast<uintptr_t>(v_pool)) & 15)
     return -141;
-  if (!pitch_fits(bt_pitch) || (ld_q & 7) || (ld_out & 7) || (reinterpret_cast<uintptr_t>(bounds) & 7)) return -142;
+  if (!pitch_fits(bt_pitch) || n_pages < 0 || (ld_q & 7) || (ld_out & 7) || (reinterpret_cast<uintptr_t>(bounds) & 7)) return -142;
   if (!shaped_scores_fit(scale, cap)) return -143;
   ShapedPromptParams p;
   p.c = shaped_cache(block_table, bt_pitch, bt_rows, n_pages, key_pos, kp_stride, bounds, slopes, scale, cap);

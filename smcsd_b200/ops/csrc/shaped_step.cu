@@ -830,7 +830,7 @@ SMC_API int smc_shaped_step(const void* q, long long ld_q, const void* k_pool, c
       (reinterpret_cast<uintptr_t>(bounds) & 7))
     return -151;
   if (!shaped_scores_fit(scale, cap)) return -152;
-  if (!pitch_fits(bt_pitch) || (mass != nullptr && mass_stride < pitch_cols(bt_pitch))) return -153;
+  if (!pitch_fits(bt_pitch) || n_pages < 0 || (mass != nullptr && mass_stride < pitch_cols(bt_pitch))) return -153;
   StepWork w = step_work(bs, E, Hq, Hkv, D, 0);
   if (mass != nullptr) w.score_tiles = (work_bytes - (long long)w.scores) / ((long long)Hkv * ((E * (Hq / Hkv) + 3) / 4 * 4) * step_tile(D) * 4);       // the rest of it
   if (work_bytes < (long long)w.bytes || (mass != nullptr && w.score_tiles < 1)) return -154;

@@ -78,7 +78,7 @@ def _rows(t: torch.Tensor, name: str, dev: int, T: int, width: int):
 
 
 def _pool(t: torch.Tensor, name: str, dev: int, width: int) -> int:
-    if t.dtype is not _BF16 or t.get_device() != dev or t.dim() != 2 or t.shape[1] != width or not t.is_contiguous():
+    if t.dtype is not _BF16 or t.get_device() != dev or t.dim() != 2 or t.shape[0] < 1 or t.shape[1] != width or not t.is_contiguous():
         raise _wrong(t, name, f"contiguous bfloat16 [pages + 1, {width}] on cuda:{dev}")
     return t.data_ptr()
 
@@ -184,7 +184,10 @@ def attention_shaped_step(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
 
 def evict_work_bytes(n_pages: int) -> int:
     """Bytes of workspace for ``evict_tokens`` on an allocator of ``n_pages`` pages (uint8, zeros at first)."""
-    return _library().smc_evict_work(n_pages)
+    n = _library().smc_evict_work(n_pages)
+    if n < 0:
+        raise ValueError(f"no allocator of {n_pages} pages")
+    return n
 
 
 def evict_tokens(block_table: torch.Tensor, src: torch.Tensor, dst: torch.Tensor, lens: torch.Tensor, mass: torch.Tensor, refcount: torch.Tensor,

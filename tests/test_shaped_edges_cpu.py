@@ -32,3 +32,16 @@ def test_pitches_are_refused_ahead_of_any_launch():
     for pitch in (0, -8, 8 | 9 << 32, 1 << 31, 1 << 40):
         assert calls(pitch) == (-142, -163, -153, -171), pitch
     assert calls(64 | 8 << 32, mass_stride=7)[1:] == (-163, -153, -171) and calls(64 | 8 << 32, kp_stride=7)[3] == -171
+
+
+@needs_library
+def test_pools_and_allocators_without_a_page_are_refused_ahead_of_any_launch():
+    """Without its scratch page a pool has no page that a bad one could be replaced by, and no workspace belongs to an allocator of nothing."""
+    L, p = N._library(), 1 << 20
+    assert L.smc_shaped_prompt(p, 512, p, p, -1, p, 8, 1, None, 0, p, 1, p, 512, None, 4, 8, 2, 64, 0.125, 0.0, None, None, p, 0, None) == -142
+    assert L.smc_shaped_mass(p, 512, p, -1, p, 8, 1, None, 0, p, 1, p, p, 8, 4, 8, 2, 64, 0.125, 0.0, None, None, p, 0, None) == -163
+    assert L.smc_shaped_step(p, 512, p, p, -1, p, 8, 1, None, 0, p, p, p, 512, None, None, 8, 2, 1, 8, 2, 64, 0.125, 0.0, None, None, p, 1 << 30, p, 0, None) == -153
+    for pages in (0, -5):
+        assert L.smc_evict(p, 8, p, 8, p, 8, p, 4, p, p, 3, 2, 8, 1, 1, p, p, p, p, pages, p, 1 << 20, p, None) == -172
+        with pytest.raises(ValueError, match="allocator"):
+            N.evict_work_bytes(pages)

@@ -375,3 +375,26 @@ def test_evict_from_a_table_of_more_columns_than_it_takes():
     assert int(st) == 0 and lens.tolist() == [0, 100] and int(count) == n - 100
     assert torch.equal(kept[0].long(), want) and torch.equal(wide[1, :100].long(), want + 1) and torch.equal(mass[1, 0, :100], before[want])
     assert not bool(mass[1, 0, 100:n].any()) and torch.equal(mass[1, 0, n:], before[n:])
+
+
+def test_evict_with_a_free_count_that_leaves_the_stack():
+    """A count below zero or above the pages: the status, and nothing written outside of the stack."""
+    N = _N()
+    for bad in (-3, 47, 60):
+        table = torch.arange(1, 51, dtype=torch.int32, device=DEV).repeat(2, 1)
+        mass, lens, st = torch.rand(2, 1, 50, device=DEV, generator=torch.Generator(DEV).manual_seed(2)), _int([0, 50]), _int([0])
+        refs = torch.ones(51, dtype=torch.int32, device=DEV)
+        stack, count, work = torch.full((150,), -9, dtype=torch.int32, device=DEV), _int([bad]), torch.zeros(N.evict_work_bytes(50), dtype=torch.uint8, device=DEV)
+        N.evict_tokens(table, _int([1]), _int([1]), lens, mass, refs, stack[50:100], count, keep=30, first=0, last=0, kept=torch.zeros(1, 30, dtype=torch.int32, device=DEV), work=work,
+                       status=st)
+        torch.cuda.synchronize()
+        assert int(st) == 8 and bool((stack[:50] == -9).all()) and bool((stack[100:] == -9).all()) and int(count) <= 50
+        assert not bool(work[:256].any()) and not bool(work[256 + 4 * 4096:].any())
+
+
+def test_arguments_without_a_page_are_refused():
+    N = _N()
+    c = Cache([20], 2, 64)
+    q, runs = torch.zeros(20, 256, dtype=torch.bfloat16, device=DEV), _int([[1, 0, 0, 20]])
+    with pytest.raises(ValueError, match="k_pool"):
+        N.attention_shaped_prompt(q, c.k[:0], c.v, c.table, runs, q.clone(), T=20, Hq=4, Hkv=2, D=64, scale=0.125, status=_int([0]))
