@@ -13,6 +13,7 @@
 namespace smc {
 
 constexpr int SH_POS_END = 1 << 24;
+constexpr float SH_TANH3_REACH = 0.35f;                // of a tanh by three or four coefficients, see below
 constexpr float SH_LOG2E = 1.4426950408889634f, SH_LN2 = 0.6931471805599453f;
 
 struct ShapedCache {
@@ -20,9 +21,11 @@ struct ShapedCache {
   const int* key_pos;            // [bt_rows, kp_stride] its position, ascending, or null
   const int2* bounds;            // per query token: first and last visible position, or null: all up to its own
   const float* slopes;           // per query head, or null
-  int bt_stride, bt_cols, bt_rows, kp_stride, n_pages;                // (a table may be some columns of a wider one)
+  int bt_stride, bt_rows, kp_stride, n_pages;
   float mul;                     // scale log2(e)
   float cap_in, cap_out;         // scale / cap and cap log2(e), 0: no cap
+  int bt_cols;                   // of the table, which may be some columns of a wider one
+  float near_reach;              // |tanh's argument| up to which factors folded into three or four coefficients serve; -1: not even zero
 };
 
 // The pitch of a block table: from row to row in the low 32 bits, its columns in the high ones (0: as many).
@@ -39,9 +42,11 @@ inline bool shaped_scores_fit(float scale, float cap) {
 // (in double precision: an error of a factor is one of every score)
 inline ShapedCache shaped_cache(const int* block_table, long long bt_pitch, int bt_rows, int n_pages, const int* key_pos, int kp_stride, const int* bounds,
                                 const float* slopes, float scale, float cap) {
-  const double log2e = 1.4426950408889634;
-  return ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, (int)pitch_stride(bt_pitch), pitch_cols(bt_pitch), bt_rows, kp_stride, n_pages, (float)(scale * log2e),
-                     cap > 0.f ? (float)((double)scale / cap) : 0.f, cap > 0.f ? (float)(cap * log2e) : 0.f};
+  const double log2e = 1.4426950408889634, in = cap > 0.f ? (double)scale / cap : 0.0;
+  // the folded coefficients hold scale log2(e) (scale / cap)^2k up to k = 3; below 2e-5 they fade
+  const float near_reach = in >= 2e-5 && scale * log2e * in * in * in * in * in * in <= 1e37 ? SH_TANH3_REACH : -1.f;
+  return ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, (int)pitch_stride(bt_pitch), bt_rows, kp_stride, n_pages, (float)(scale * log2e),
+                     cap > 0.f ? (float)((double)scale / cap) : 0.f, cap > 0.f ? (float)(cap * log2e) : 0.f, pitch_cols(bt_pitch), near_reach};
 }
 
 // One sequence of a call: block-table row, tokens held before the new ones, index of the first new one in q, new tokens.
@@ -144,7 +149,7 @@ __device__ __forceinline__ float shaped_min3(float a, float b, float c) {
 // tanh u = u P(u^2): minimax polynomials of tanh(sqrt y) / sqrt y on [0, reach^2], found by an exchange algorithm in double precision.
 // Largest relative errors: three coefficients up to 0.35 2.8e-6, five up to 0.75 5.2e-7 (behind these two stand probabilities of eight bits);
 // four up to 0.35 3.4e-8, six up to 0.625 3.7e-9 (32-bit results).  Scores beyond, rare at the usual caps, take 1 - 2 / (1 + e^2|u|).
-constexpr float SH_TANH3_REACH = 0.35f, SH_TANH5_REACH = 0.75f, SH_TANH6_REACH = 0.625f;
+constexpr float SH_TANH5_REACH = 0.75f, SH_TANH6_REACH = 0.625f;
 template <int N>
 __host__ __device__ constexpr float tanh_coef(int k) {
   constexpr float c3[3] = {0.9999971985816956f, -0.33291319012641907f, 0.1239800825715065f};
@@ -172,11 +177,10 @@ __device__ __forceinline__ float shaped_cap(float x, float in, float out) {
   return t * out;
 }
 // out tanh(x in) + add of two numbers within reach.  With three or four coefficients the factors are folded into them (N + 1 operations a pair); where the
-// powers of `in` leave the range of fp32 the reach is nothing, not even zero.  With more, u is made first.
+// powers of `in` leave the range of fp32 (near_reach: -1) it does not serve.  With more, u is made first.
 template <int N>
 struct ShapedCapNear {
   uint64_t c[N], in2;
-  float reach;
   __device__ __forceinline__ ShapedCapNear(float in, float out, float in_out) {
     float f = N <= 4 ? in_out : out;
 #pragma unroll
@@ -185,7 +189,6 @@ struct ShapedCapNear {
       if (N <= 4) f *= in * in;
     }
     in2 = f2_pair(in, in);
-    reach = N <= 4 ? (in >= 2e-5f && f <= 1e38f ? SH_TANH3_REACH : -1.f) : N == 5 ? SH_TANH5_REACH : SH_TANH6_REACH;
   }
   __device__ __forceinline__ uint64_t operator()(uint64_t x, uint64_t add) const {
     const uint64_t u = N <= 4 ? x : f2_mul(x, in2), y = f2_mul(u, u);

@@ -405,7 +405,7 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
             float far = 0.f;
 #pragma unroll
             for (int i = 0; i < 64; i += 2) far = shaped_max3(far, fabsf(__uint_as_float(w[i >> 5][i & 31])), fabsf(__uint_as_float(w[i >> 5][(i & 31) + 1])));
-            reach = __all_sync(0xffffffffu, far * cap_in <= near.reach);
+            reach = __all_sync(0xffffffffu, far * cap_in <= p.c.near_reach);
           }
           if (full && reach && behind) {
 #pragma unroll

@@ -474,7 +474,7 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
       // 0: scores as they are after this; 1: tanh by three coefficients (or none); 2: by five
       int way = 1;
       if (!plain || (BIAS && __any_sync(0xffffffffu, !((most - least) * mul < 60.f)))) way = 0;
-      else if (CAP && __any_sync(0xffffffffu, !(reach <= near.reach))) way = __any_sync(0xffffffffu, !(reach <= SH_TANH5_REACH)) ? 0 : 2;
+      else if (CAP && __any_sync(0xffffffffu, !(reach <= p.c.near_reach))) way = __any_sync(0xffffffffu, !(reach <= SH_TANH5_REACH)) ? 0 : 2;
       float top;
       if (way != 0) {
         top = CAP ? shaped_cap(most, cap_in, cap_out) : most * mul;
