@@ -96,7 +96,7 @@ __device__ __forceinline__ void sp_umma_ts(uint32_t tmem_d, uint32_t tmem_a, uin
 // Tile number `want` (0: most steps) of all tiles of `tokens` tokens, by a whole warp; run number and tile inside it, or false behind the
 // last.  The tiles of a sequence with at least c steps of `bk` keys are its last ones, so counting them is arithmetic and c of the
 // wanted one is found by bisection.
-__device__ __forceinline__ bool sp_find_tile(const ShapedCache& c, const int4* runs, int n_runs, int T, int* status, int tokens, int bk, int want,
+__device__ __forceinline__ bool sp_find_tile(const ShapedCache& c, const int4* runs, int n_runs, int T, int* status, int tokens, int bk, int launched, int want,
                                              ShapedRun& run, int& tile) {
   const int lane = threadIdx.x & 31;
   const ShapedRun mine = lane < n_runs ? shaped_run(c, runs, lane, T, status) : ShapedRun{0, 0, 0, 0};
@@ -111,7 +111,9 @@ __device__ __forceinline__ bool sp_find_tile(const ShapedCache& c, const int4* r
     for (int s = lane + 32; s < n_runs; s += 32) n += of_run(shaped_run(c, runs, s, T, status), cost);
     return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
   };
-  if (count(1) <= want) return false;
+  const int tiles = count(1);
+  if (tiles > launched && want == 0 && threadIdx.x == 0) atomicOr(status, SMC_ERR_BOUNDS);      // tokens of q in two runs: more tiles than q has
+  if (tiles <= want) return false;
   int lo = 1, hi = c.bt_cols / bk + 2;                                // count(lo) > want >= count(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -171,7 +173,7 @@ shaped_prompt_kernel(const ShapedPromptParams p, const __grid_constant__ CUtenso
 
   ShapedRun run;
   int tile;
-  if (!sp_find_tile(p.c, p.runs, p.n_runs, p.T, p.status, NT * TT, BK, blockIdx.x / p.Hkv, run, tile)) return;
+  if (!sp_find_tile(p.c, p.runs, p.n_runs, p.T, p.status, NT * TT, BK, gridDim.x / p.Hkv, blockIdx.x / p.Hkv, run, tile)) return;
   const int first = run.held + tile * NT * TT, tok0 = run.at + tile * NT * TT;       // index in the row and in q of the first token
   const int count = min(NT * TT, run.n - tile * NT * TT), keys = run.held + run.n;
   const int* kp = p.c.key_pos != nullptr ? p.c.key_pos + (size_t)run.row * p.c.kp_stride : nullptr;

@@ -13,8 +13,8 @@ and a log-sum-exp of -inf.  ``scale``, ``softcap`` and ``scale / softcap`` have 
 The cache is the block table's: one page per token, bf16 rows of Hkv * D values (the e4m3 cache is refused), all tokens of a call
 already written.  ``key_pos`` lists the positions of a row's tokens, ascending and below 2^24, once tokens have been shed; without it token j
 of a row has position j.  The weights live in ``mass`` [rows, Hkv, tokens], fp32, beside the block table; entries behind a row's last
-token are zero.  A key or value that is not finite spoils the tokens that share a tile of queries (up to 128 rows
-of tokens x heads) with one that sees it; cached tokens outside the span of a tile's intervals are not read.
+token are zero.  A key or value that is not finite spoils the tokens that share a tile of queries with one that sees
+it (prompts: up to 256 rows of tokens x heads, 128 with heads of 256; steps: those of the sequence); cached tokens outside the span of a tile's intervals are not read.
 
 As everywhere, calls run on the current stream, allocate nothing and can be captured; ``status`` collects error bits.  Two calls that may
 run at the same time need a workspace each.
@@ -144,7 +144,8 @@ def attention_key_mass(q: torch.Tensor, k_pool: torch.Tensor, block_table: torch
                        Hq: int, Hkv: int, D: int, scale: float, status: torch.Tensor, softcap: float = 0.0, slopes: Optional[torch.Tensor] = None,
                        bounds: Optional[torch.Tensor] = None, key_pos: Optional[torch.Tensor] = None, pdl: bool = False) -> None:
     """``mass[row, kv head, j]`` += the attention weight that token j of the row gets from the tokens and query heads of the pass that left ``lse``
-    (same arguments).  ``runs`` may list fewer tokens than that pass - the last ones of a prompt, say - but a row only once."""
+    (same arguments).  ``runs`` may list fewer tokens than that pass - the last ones of a prompt, say - but a row only once, and tokens of the row behind the last listed
+    one get nothing."""
     L, dev = _library(), _device(q)
     qp, ldq = _rows(q, "q", dev, T, Hq * D)
     (bt, bts, rows), (kp, kps) = _tables(block_table, key_pos, dev)

@@ -398,3 +398,15 @@ def test_arguments_without_a_page_are_refused():
     q, runs = torch.zeros(20, 256, dtype=torch.bfloat16, device=DEV), _int([[1, 0, 0, 20]])
     with pytest.raises(ValueError, match="k_pool"):
         N.attention_shaped_prompt(q, c.k[:0], c.v, c.table, runs, q.clone(), T=20, Hq=4, Hkv=2, D=64, scale=0.125, status=_int([0]))
+
+
+# ------------------------------------------------------------------------------- runs that share tokens
+def test_more_tiles_than_the_queries_have_raise_the_status():
+    """Tokens of ``q`` in several runs make more tiles than are launched: some would be left out without a word.  Runs that fill the queries exactly are fine."""
+    N = _N()
+    c = Cache([100] * 5, 2, 64, seed=30)
+    q = _randn(100, 8 * 64, seed=31)
+    for runs, want in (([[i + 1, 0, 0, 100] for i in range(5)], 8), ([[1, 0, 0, 65], [2, 0, 65, 1], [3, 0, 66, 1], [4, 0, 67, 1], [5, 0, 68, 32]], 0)):
+        st = _int([0])
+        N.attention_shaped_prompt(q, c.k, c.v, c.table, _int(runs), torch.zeros_like(q), T=100, Hq=8, Hkv=2, D=64, scale=0.125, status=st)
+        assert int(st) == want
