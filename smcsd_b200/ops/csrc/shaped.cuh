@@ -100,14 +100,6 @@ __device__ __forceinline__ float shaped_ex2(float x) {
 template <int N> __device__ __forceinline__ void regs_fewer() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// one column of tensor memory, a number per lane
-__device__ __forceinline__ void tmem_ld_32x32b_x1(uint32_t taddr, uint32_t& r) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
-}
-__device__ __forceinline__ void tmem_st_32x32b_x1(uint32_t taddr, uint32_t r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r));
-}
-
 // two fp32 operations at once
 __device__ __forceinline__ uint64_t f2_pair(float a, float b) {
   uint64_t y;
@@ -147,8 +139,9 @@ __device__ __forceinline__ float shaped_min3(float a, float b, float c) {
 }
 
 // tanh u = u P(u^2): minimax polynomials of tanh(sqrt y) / sqrt y on [0, reach^2], found by an exchange algorithm in double precision.
-// Largest relative errors: three coefficients up to 0.35 2.8e-6, five up to 0.75 5.2e-7 (behind these two stand probabilities of eight bits);
-// four up to 0.35 3.4e-8, six up to 0.625 3.7e-9 (32-bit results).  Scores beyond, rare at the usual caps, take 1 - 2 / (1 + e^2|u|).
+// Largest relative errors, of the coefficients as they stand here in fp32: three up to 0.35 3.0e-6, five up to 0.75 6.3e-7 (the probabilities behind these two are rounded to
+// eight bits, but the log-sum-exp of a prompt takes them along: up to 0.35 x 3.0e-6 of a cap, 5e-5 at 50; four and six in their place 8192 tokens 772 -> 872 us);
+// four up to 0.35 6.1e-8, six up to 0.625 1.0e-8 (32-bit results).  Scores beyond, rare at the usual caps, take 1 - 2 / (1 + e^2|u|).
 constexpr float SH_TANH5_REACH = 0.75f, SH_TANH6_REACH = 0.625f;
 template <int N>
 __host__ __device__ constexpr float tanh_coef(int k) {

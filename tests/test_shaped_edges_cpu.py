@@ -1,6 +1,8 @@
 """Shaped attention at its edges, as far as that goes without a GPU."""
 import os
+import re
 
+import numpy as np
 import pytest
 
 from smcsd_b200.ops import native as K
@@ -45,3 +47,14 @@ def test_pools_and_allocators_without_a_page_are_refused_ahead_of_any_launch():
         assert L.smc_evict(p, 8, p, 8, p, 8, p, 4, p, p, 3, 2, 8, 1, 1, p, p, p, p, pages, p, 1 << 20, p, None) == -172
         with pytest.raises(ValueError, match="allocator"):
             N.evict_work_bytes(pages)
+
+
+def test_polynomials_of_the_tanh_are_as_close_as_their_header_says():
+    """Relative to tanh, over the reach of each, with the coefficients rounded to fp32 as the kernels have them."""
+    text = open(os.path.join(os.path.dirname(K.__file__), "csrc", "shaped.cuh")).read()
+    for n, reach, off in ((3, 0.35, 3.0e-6), (4, 0.35, 6.1e-8), (5, 0.75, 6.3e-7), (6, 0.625, 1.0e-8)):
+        coef = [np.float64(np.float32(float(x.rstrip("f")))) for x in re.search(r"c%d\[%d\] = \{([^}]*)\}" % (n, n), text).group(1).split(",")]
+        u = np.linspace(1e-4, reach, 400001)
+        got = u * sum(c * u ** (2 * k) for k, c in enumerate(coef))
+        worst = np.abs(got / np.tanh(u) - 1).max()
+        assert len(coef) == n and 0.9 * off <= worst <= off, (n, worst)

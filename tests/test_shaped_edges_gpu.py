@@ -410,3 +410,30 @@ def test_more_tiles_than_the_queries_have_raise_the_status():
         st = _int([0])
         N.attention_shaped_prompt(q, c.k, c.v, c.table, _int(runs), torch.zeros_like(q), T=100, Hq=8, Hkv=2, D=64, scale=0.125, status=st)
         assert int(st) == want
+
+
+# ------------------------------------------------------------------------------- 32-bit results
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (8, 2, 128), (8, 1, 256)])
+@pytest.mark.parametrize("softcap", [0.0, 50.0])
+@pytest.mark.parametrize("alibi", [False, True])
+def test_weights_and_log_sums_keep_their_32_bits(Hq, Hkv, D, softcap, alibi):
+    """Root mean squares, beside the worst cases of the other tests.  A score is summed in D / 16 additions, each off by at most 2^-23 of the sum so far, itself no more than a few
+    scores; its tanh is off by 6.1e-8 (a log-sum-exp of a prompt's by 3.0e-6 up to 0.35 of the cap and 6.3e-7 beyond), an exponential by 2^-22, a log-sum-exp by 2^-24 of itself."""
+    N = _N()
+    n, scale = 700, D ** -0.5
+    c = Cache([n], Hkv, D, seed=41)
+    q, st = (1.6 * _randn(n, Hq * D, seed=42).float()).bfloat16(), _int([0])
+    kw = dict(scale=scale, softcap=softcap, slopes=_slopes(Hq) if alibi else None)
+    _, want_lse, mass = attend(c, [(1, 0, 0, n)], q, Hq, **kw)
+    out, lse, m = torch.zeros_like(q), torch.zeros(n, Hq, device=DEV), torch.zeros(2, Hkv, c.table.shape[1], device=DEV)
+    kw.update(T=n, Hq=Hq, Hkv=Hkv, D=D, status=st)
+    N.attention_shaped_prompt(q, c.k, c.v, c.table, _int([[1, 0, 0, n]]), out, lse=lse, **kw)
+    N.attention_key_mass(q, c.k, c.table, _int([[1, 0, 0, n]]), want_lse.float(), m, **kw)
+    torch.cuda.synchronize()
+    score = 1.6                                                      # root mean square of q.k scale, for keys of unit variance
+    moved = D / 16 * 2.0 ** -23 * 2 * score + 2.0 ** -22 + 2.0 ** -24 * float(want_lse.abs().max())
+    off = (m[1, :, :n].double() - mass[1]) / mass[1]
+    assert int(st) == 0 and float(off.pow(2).mean().sqrt()) <= moved + (6.1e-8 * 4 * score if softcap else 0.0)
+    diff = lse.double() - want_lse
+    tanh = max(3.0e-6 * 0.35, 6.3e-7 * 0.75) * softcap
+    assert float(diff.pow(2).mean().sqrt()) <= moved + tanh / 2 and float(diff.abs().max()) <= 8 * moved + tanh
