@@ -24,7 +24,7 @@ struct ShapedCache {
   int bt_stride, bt_rows, kp_stride, n_pages;
   float mul;                     // scale log2(e)
   float cap_in, cap_out;         // scale / cap and cap log2(e), 0: no cap
-  int bt_cols;                   // of the table, which may be some columns of a wider one
+  int bt_cols;                   // of the table, which may be some columns of a wider one; those that a position can name
   float near_reach;              // |tanh's argument| up to which factors folded into three or four coefficients serve; -1: not even zero
 };
 
@@ -46,7 +46,8 @@ inline ShapedCache shaped_cache(const int* block_table, long long bt_pitch, int 
   // the folded coefficients hold scale log2(e) (scale / cap)^2k up to k = 3; below 2e-5 they fade
   const float near_reach = in >= 2e-5 && scale * log2e * in * in * in * in * in * in <= 1e37 ? SH_TANH3_REACH : -1.f;
   return ShapedCache{block_table, key_pos, (const int2*)bounds, slopes, (int)pitch_stride(bt_pitch), bt_rows, kp_stride, n_pages, (float)(scale * log2e),
-                     cap > 0.f ? (float)((double)scale / cap) : 0.f, cap > 0.f ? (float)(cap * log2e) : 0.f, pitch_cols(bt_pitch), near_reach};
+                     cap > 0.f ? (float)((double)scale / cap) : 0.f, cap > 0.f ? (float)(cap * log2e) : 0.f,
+                     pitch_cols(bt_pitch) < SH_POS_END ? pitch_cols(bt_pitch) : SH_POS_END, near_reach};
 }
 
 // One sequence of a call: block-table row, tokens held before the new ones, index of the first new one in q, new tokens.

@@ -78,7 +78,7 @@ __device__ __forceinline__ void step_spans(const ShapedStepParams& p, const Step
     if (s < p.bs) {
       row = p.rows[s];
       len = p.lens[s];
-      if (row < 0 || row >= p.c.bt_rows || len < 0 || len > min(p.c.bt_cols, SH_POS_END)) {
+      if (row < 0 || row >= p.c.bt_rows || len < 0 || len > p.c.bt_cols) {
         atomicOr(p.status, SMC_ERR_BOUNDS);
         row = len = 0;
       }

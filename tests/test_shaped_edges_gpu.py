@@ -437,3 +437,19 @@ def test_weights_and_log_sums_keep_their_32_bits(Hq, Hkv, D, softcap, alibi):
     diff = lse.double() - want_lse
     tanh = max(3.0e-6 * 0.35, 6.3e-7 * 0.75) * softcap
     assert float(diff.pow(2).mean().sqrt()) <= moved + tanh / 2 and float(diff.abs().max()) <= 8 * moved + tanh
+
+
+def test_rows_of_more_tokens_than_positions_raise_the_status():
+    N = _N()
+    n = 2 ** 24
+    table = torch.ones(1, n + 8, dtype=torch.int32, device=DEV)
+    pool, q = torch.ones(2, 64, dtype=torch.bfloat16, device=DEV), torch.ones(1, 64, dtype=torch.bfloat16, device=DEV)
+    work = torch.zeros(N.shaped_step_work_bytes(1, 1, 1, 1, 64), dtype=torch.uint8, device=DEV)
+    kw = dict(Hq=1, Hkv=1, D=64, scale=0.125)
+    for keys, want in ((n, 0), (n + 1, 8)):
+        last = _int([[keys - 200, keys - 1]])
+        for call in (lambda st, o: N.attention_shaped_prompt(q, pool, pool, table, _int([[0, keys - 1, 0, 1]]), o, T=1, status=st, bounds=last, **kw),
+                     lambda st, o: N.attention_shaped_step(q, pool, pool, table, _int([0]), _int([keys]), o, bs=1, E=1, work=work, status=st, bounds=last, **kw)):
+            st, out = _int([0]), torch.zeros_like(q)
+            call(st, out)
+            assert int(st) == want and bool((out == (0.0 if want else 1.0)).all())
