@@ -453,3 +453,25 @@ def test_rows_of_more_tokens_than_positions_raise_the_status():
             st, out = _int([0]), torch.zeros_like(q)
             call(st, out)
             assert int(st) == want and bool((out == (0.0 if want else 1.0)).all())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 64), (16, 4, 128), (16, 2, 256)])
+def test_distance_bias_across_a_gap_ahead_of_the_tokens(Hq, Hkv, D):
+    """Tokens that see all others, of which many lie behind a gap: the first key of a step is the nearest one then."""
+    N = _N()
+    n, gap = 600, 10 ** 6
+    for ahead in (130, 390):
+        c = _gap_cache([n], Hkv, D, ahead, gap, seed=ahead)
+        q, st = _randn(n, Hq * D, seed=D), _int([0])
+        bounds = _int([[0, 2 ** 24 - 1]] * n)
+        kw = dict(scale=D ** -0.5, slopes=_slopes(Hq), bounds=bounds)
+        want, want_lse, mass = attend(c, [(1, 0, 0, n)], q, Hq, **kw)
+        out, lse, m = torch.zeros_like(q), torch.zeros(n, Hq, device=DEV), torch.zeros(2, Hkv, c.table.shape[1], device=DEV)
+        kw.update(T=n, Hq=Hq, Hkv=Hkv, D=D, status=st, key_pos=c.key_pos)
+        N.attention_shaped_prompt(q, c.k, c.v, c.table, _int([[1, 0, 0, n]]), out, lse=lse, **kw)
+        N.attention_key_mass(q, c.k, c.table, _int([[1, 0, 0, n]]), want_lse.float(), m, **kw)
+        torch.cuda.synchronize()
+        moved = _score_error(c, q, D ** -0.5) + 2.0 ** -20
+        assert int(st) == 0 and float((lse.double() - want_lse).abs().max()) <= moved
+        assert float((out.double().view(want.shape) - want).abs().max()) <= _out_error(c, moved)
+        assert bool(((m[1, :, :n].double() - mass[1]).abs() <= 2 * moved * mass[1] + 1e-12).all())
