@@ -8,8 +8,8 @@
 //     S_t = K_t Q^T      UMMA 128 x 128 x D, two buffers per key tile in tensor memory
 //     sum                four warps per key tile: exp2(x - lse) of 128 columns, masked by the key's position where a column does not see all keys
 // What bounds it is the exponential, one per (token, head, key) pair; the product is half of the attention's.  A step of 128 columns takes 2700 cycles of the 2048 its
-// exponentials take on the two warps of a scheduler, 4400 with a cap; a key tile 8 us from its pages to its first sum.  Microseconds on B200: 4096 tokens of 32 heads on
-// 8: heads of 128 128, capped 200, distance bias and cap 226; the last 33 to 64 tokens of four prompts of 20,000, heads of 64 117.
+// exponentials take on the two warps of a scheduler, 4400 with a cap; a key tile 8 us from its pages to its first sum.  Microseconds on B200 (device times,
+// graphs replayed): 4096 tokens of 32 heads on 8: heads of 128 133, capped 202, distance bias 154, both 235; the last 33 to 64 tokens of four prompts of 20,000, heads of 64 119.
 // The grid is persistent: key tiles of all sequences, those with most tokens behind them first; the next tile's keys are fetched while one is worked on.  Where sequences bring
 // many tokens the two blocks of a cluster take the steps of a tile by turns and add up their sums through shared memory in their order.
 #include <atomic>

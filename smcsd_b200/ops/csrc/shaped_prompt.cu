@@ -8,8 +8,9 @@
 //     O_t += P_t V       UMMA 128 x D x BK accumulating in tensor memory, P its left operand there
 // m_ref moves only when the row maximum has grown by more than 2^8.  Sums stay in fp32 ahead of the rounding of P to bf16.
 // The shape of the scores costs little beside the exponential: a tanh is a polynomial whose last operation also takes the reference off (four
-// operations a pair of scores instead of one), a distance is linear over a step and one operation more; only steps that a row sees in part, and scores
-// far beyond the polynomial, are shaped number by number.  (Shaped in a pass of their own ahead of the maximum: 8192 tokens capped 986 us, folded 774.)
+// operations a pair of scores instead of one), a distance is linear over a step from its nearest key on and one operation more; only steps that a row sees in part, and
+// scores far beyond the polynomial, are shaped number by number.  (Shaped in a pass of their own ahead of the maximum: 8192 tokens capped 986 us, folded 772.)  What a
+// tanh still costs is in part registers: with heads of 64 and 128 the capped variants spill some 350 bytes a thread, the others up to 12.
 //
 // What bounds it is the chain of a step: 4700 cycles for 128 keys and two row tiles, of which the exponentials take 2048 and the products, with heads of
 // 128, 2048.  A row tile waits 1750 cycles for P V and the next scores (the second waits for the first: the probabilities lie over
@@ -17,8 +18,9 @@
 // P goes to the tensor cores while the second is made.  Taken back: half a row per thread on twice the warps (heads of 128 654 -> 785 us, of 64 555 -> 523),
 // steps of 64 keys with two score buffers and the next scores shaped between the exponentials (654 -> 810), probabilities beside the scores for heads of
 // 64 and 256 (555 -> 586, 658 -> 849), a quarter of the exponentials by polynomial (610 -> 600).
-// Microseconds on B200, 8192 causal tokens: 32/8 heads of 128 646 (0.85 PFLOP/s), capped 774, distance bias 797; of 64 554 and 695; 16/2 heads of 256 719 and 859.  Tokens
-// behind a thinned-out cache (pages in any order): two portions of 411 and 512 behind 6000, heads of 256, 62; three turns of 37 to 181 tokens 16.5, of them 4.5 until the first scores.
+// Microseconds on B200 (device times, graphs replayed), 8192 causal tokens: 32/8 heads of 128 646 (0.85 PFLOP/s), capped 772, distance bias 811, both 941; of 64 553 and 687 capped;
+// 16/2 heads of 256 719 and 871.  Tokens behind a thinned-out cache (pages in any order): two portions of 411 and 512 behind 6000, heads of 256, 63; three turns of 37 to 181
+// tokens 17, of them 4.5 until the first scores.
 // Tiles are found on the device, the longest walks first: nothing but the number of tokens and sequences has to be known at the launch.
 // Every mbarrier wait is bounded; a timeout raises a status bit and all roles unwind.
 #include "shaped.cuh"

@@ -8,12 +8,12 @@
 //
 // Keys are the rows of the products (mma.sync, 16 x 8 x 16) and queries their eight columns: S^T = K Q^T and O^T += V^T P^T, so that the
 // four or eight heads of a group fill a fragment (as rows of sixteen they left half of every product and of the softmax idle: heads of 256, 4 x 57,600 keys
-// 110 -> 96 us).  tcgen05 has no such narrow form: its 128 lanes would hold keys, and the softmax would run across lanes.  From 17 rows on
-// the products cost more than the cache: 36 rows (nine tokens of groups of four) take 2.7 times as long as four on the same keys.
+// 110 -> 96 us).  tcgen05 has no such narrow form: with keys in its 128 lanes the softmax would run across lanes, with queries there most of them would be empty.  From 17 rows
+// on the products cost more than the cache: 36 rows (nine tokens of groups of four) take 2.7 times as long as four on the same keys.
 //
-// Microseconds on B200 (of them at the measured 6.54 TB/s): 4 x 57,600 keys, 8 KV heads of 128, groups of four: 154 (145); of 64: 91 (72); 2 heads of 256: 83 (72); with the
-// mass, 48 sequences of 600 to 9000 keys: 190 (147), two of 99,000 and 131,000: 185 (147); one sequence of 701 keys, heads of 64: 9.3, a launch, three dependent reads and a
-// join.  Rows of 512 bytes as bulk copies 96 -> 87, the cache's lines first out of L2 157 -> 154 and 196 -> 190 with the mass.
+// Microseconds on B200 (device times, graphs replayed; of them at the measured 6.54 TB/s): 4 x 57,600 keys, 8 KV heads of 128, groups of four: 156 (145); of 64: 91 (72); 2 heads of
+// 256: 83 (72); with the mass, 48 sequences of 600 to 9000 keys: 190 (147), two of 99,000 and 131,000: 184 (147); a window of 2048 over the 48, thinned out, without the mass:
+// 42 (19); one sequence of 701 keys, heads of 64: 9.3, a launch, three dependent reads and a join.  Rows of 512 bytes as bulk copies 96 -> 87, the cache's lines first out of L2 157 -> 154 and 196 -> 190 with the mass.
 //
 // Where a sequence ends inside a worker's part its state goes to the workspace, and the worker that comes last joins the
 // parts of a (sequence, KV head) in the order of its keys, so that results do not depend on the order of arrival.
