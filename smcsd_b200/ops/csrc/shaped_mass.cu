@@ -278,8 +278,9 @@ __global__ void __launch_bounds__((5 * MsCfg<D>::NT + MS_LOADERS) * 32, 1) shape
         MsColumns& col = S.col[u % SLOTS];
         col.neg_lse[cl] = nl;
         col.pos[cl] = posf;
-        col.first[cl] = first;
-        col.last[cl] = last;
+        // columns without a token see nothing (a key that is not finite makes NaN of their zeros), but do not send their step the long way
+        col.first[cl] = live ? first : (float)SH_POS_END;
+        col.last[cl] = live ? last : -1.f;
         if (BIAS) col.slope[cl] = slope;
         const float mf = warp_max(first), ml = -warp_max(-last);
         const float mp = BIAS ? -warp_max(live ? -posf : -(float)SH_POS_END) : 0.f;

@@ -475,3 +475,39 @@ def test_distance_bias_across_a_gap_ahead_of_the_tokens(Hq, Hkv, D):
         assert int(st) == 0 and float((lse.double() - want_lse).abs().max()) <= moved
         assert float((out.double().view(want.shape) - want).abs().max()) <= _out_error(c, moved)
         assert bool(((m[1, :, :n].double() - mass[1]).abs() <= 2 * moved * mass[1] + 1e-12).all())
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(32, 8, 64), (16, 4, 128), (16, 2, 256)])
+@pytest.mark.parametrize("shed", [False, True])
+@pytest.mark.parametrize("softcap,alibi", [(0.0, False), (20.0, True)])
+def test_prompts_take_nothing_from_outside_of_the_intervals(Hq, Hkv, D, shed, softcap, alibi):
+    """Keys and values that no token of their sequence sees are NaN, ahead of a window, behind where the masks end, and in a sequence whose masks are all empty."""
+    N = _N()
+    sizes = [(900, 50), (300, 200), (400, 30), (64, 40)]
+    c, clean = (Cache([a + n for a, n in sizes], Hkv, D, seed=D, shed=shed) for _ in range(2))
+    runs, b, at = [], [], 0
+    for i, (held, n) in enumerate(sizes):
+        pos = c.positions(i + 1)
+        own, last = pos[held:], int(pos[-1])
+        see = (N.score_bounds(own, window=100), _int([[last // 4, last // 2]] * n), N.score_bounds(own, doc_first=torch.full_like(own, int(pos[min(200, len(pos) - 1)]))), _int([[9, 8]] * n))[i]
+        some = see[see[:, 0] <= see[:, 1]]
+        unseen = (pos < some[:, 0].min()) | (pos > some[:, 1].max()) if len(some) else torch.ones_like(pos, dtype=torch.bool)
+        hidden = c.table[i + 1, :held + n][unseen].long()
+        c.k[hidden] = c.v[hidden] = float("nan")
+        runs.append((i + 1, held, at, n))
+        b.append(see)
+        at += n
+    b, q, st, scale = torch.cat(b).contiguous(), _randn(at, Hq * D, seed=3), _int([0]), D ** -0.5
+    kw = dict(scale=scale, softcap=softcap, slopes=_slopes(Hq) if alibi else None, bounds=b)
+    want, want_lse, mass = attend(clean, runs, q, Hq, **kw)
+    out, lse, m = torch.full_like(q, 7.0), torch.zeros(at, Hq, device=DEV), torch.zeros(5, Hkv, c.table.shape[1], device=DEV)
+    kw.update(T=at, Hq=Hq, Hkv=Hkv, D=D, status=st, key_pos=c.key_pos)
+    N.attention_shaped_prompt(q, c.k, c.v, c.table, _int(runs), out, lse=lse, **kw)
+    N.attention_key_mass(q, c.k, c.table, _int(runs), lse, m, **kw)
+    torch.cuda.synchronize()
+    moved = _score_error(clean, q, scale) + 3e-6 * softcap + 2.0 ** -20
+    there = torch.isfinite(want_lse)
+    assert int(st) == 0 and float((out.double().view(want.shape) - want).abs().max()) <= _out_error(clean, moved)
+    assert torch.equal(torch.isfinite(lse), there) and float((lse.double() - want_lse)[there].abs().max()) <= moved
+    for row, w in mass.items():
+        assert bool(((m[row, :, :w.shape[1]].double() - w).abs() <= 2 * moved * w + 1e-12).all())
